@@ -151,11 +151,15 @@ def _cost_gemm(out, x, w, *args, **kw):
 
 
 def _cost_attention(out, q, k_pages, *args, **kw):
+    """What attention over pages of keys and of values moves and computes."""
+    return _attention_cost(out, q, 2 * k_pages.shape[1] * q.shape[2] * k_pages.element_size(), **kw)
+
+
+def _attention_cost(out, q, token_bytes: int, **kw):
     """Keys and values of the live sequences once, q in, the result out; flops of
     the two products over the keys every query row sees (lengths are on the
     device: they are read when the report is made)."""
     nq, D = q.shape[1], q.shape[2]
-    nkv, item = k_pages.shape[1], k_pages.element_size()
     kv_len, slots, cu_q, window = kw.get("kv_len"), kw.get("slots"), kw.get("cu_q"), kw.get("window")
     chunk = kw.get("chunk")
     if kv_len is None:
@@ -175,7 +179,7 @@ def _cost_attention(out, q, k_pages, *args, **kw):
         pairs = tri(lens) - tri(lens - rows)
         first = torch.clamp(lens - rows, min=0)
         lens = lens - torch.floor(first / chunk) * chunk
-    kv_bytes = (lens.sum() * (2 * nkv * D * item))
+    kv_bytes = lens.sum() * token_bytes
     pair_sum = pairs.sum()
     base = _nbytes(q, out)
     return (lambda: base + float(kv_bytes.item())), (lambda: 4.0 * nq * D * float(pair_sum.item()))
@@ -1791,6 +1795,351 @@ def attention(q, k_pages, v_pages, block_table, *, step, page: int, scale: float
     return attn_generic(q, k_pages, v_pages, block_table, token_seq=step.token_seq,
                         token_pos=step.token_pos, slots=step.slots, page=page, scale=scale,
                         window=window, **extra)
+
+
+# ---------------------------------------------------------------- a cache in 4 bits
+_TC_ERROR_NAMES[141] = "a warp of the 4-bit decode attention waited 2 s for keys that never arrived"
+KV4_PAGE = 64              # tokens of a page
+
+
+def kv4_record(D: int) -> int:
+    """Bytes of a record: 16 tokens' keys and values of one kv head of D elements (64 or 128), 4 bits each,
+    and a pair of bfloat16 (step, least) for every 64 of them."""
+    if D not in (64, 128):
+        raise KernelError(f"a cache in 4 bits has heads of 64 or 128, not {D}")
+    return 18 * D
+
+
+def kv4_pages(n_pages: int, nkv: int, D: int, device) -> torch.Tensor:
+    """Pages of a 4-bit cache, uint8 [pages, kv heads, 4, record]: 64 tokens of every kv head as four records."""
+    return torch.zeros((n_pages, nkv, 4, kv4_record(D)), dtype=torch.uint8, device=device)
+
+
+def _kv4_pages_of(pages, device=None):
+    """(pages, kv heads, D) of a 4-bit cache's pages."""
+    _need(pages, "4-bit pages", torch.uint8, 4)
+    n, nkv, four, record = pages.shape
+    if four != 4 or record not in (18 * 64, 18 * 128) or n < 1 or nkv < 1 or pages.data_ptr() % 16:
+        raise KernelError(f"4-bit pages are {tuple(pages.shape)}, expected [pages, kv heads, 4, {18 * 64} or {18 * 128}]")
+    return n, nkv, record // 18
+
+
+def _same_device(t: torch.Tensor, *others) -> None:
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise KernelError(f"tensors on {t.device} and on {o.device}")
+
+
+def _on(t: torch.Tensor):
+    """The tensor's device made the current one, so that the launch goes to its current stream."""
+    return torch.cuda.device(t.device)
+
+
+class _Kv4RowsArgs(ctypes.Structure):
+    _fields_ = [("kv", _P), ("out", _P), ("token_seq", _P), ("token_pos", _P), ("slots", _P), ("block_table", _P),
+                ("pages", _P), ("weights", _P), ("T", _I), ("n_seqs", _I), ("n_slots", _I), ("nkv", _I),
+                ("max_pages", _I), ("n_pages", _I)]
+
+
+def _kv4_rows_args(pages, weights, token_seq, token_pos, slots, block_table, page: int):
+    n_pages, nkv, D = _kv4_pages_of(pages)
+    if page != KV4_PAGE:
+        raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
+    for t, nm in ((token_seq, "token_seq"), (token_pos, "token_pos"), (slots, "slots")):
+        _need(t, nm, torch.int32, 1)
+    _need(block_table, "block table", torch.int32, 2)
+    if token_pos.shape[0] != token_seq.shape[0]:
+        raise KernelError(f"{token_seq.shape[0]} tokens have {token_pos.shape[0]} positions")
+    if weights is not None:
+        _check_kv4_weights(weights, pages)
+    _same_device(pages, token_seq, token_pos, slots, block_table, weights)
+    a = _Kv4RowsArgs()
+    a.token_seq, a.token_pos, a.slots = token_seq.data_ptr(), token_pos.data_ptr(), slots.data_ptr()
+    a.block_table, a.pages, a.weights = block_table.data_ptr(), pages.data_ptr(), _ptr(weights)
+    a.T, a.n_seqs, a.n_slots, a.nkv = token_seq.shape[0], slots.shape[0], block_table.shape[0], nkv
+    a.max_pages, a.n_pages = block_table.shape[1], n_pages
+    return a, nkv, D
+
+
+def _check_kv4_weights(weights, pages) -> None:
+    _need(weights, "token weights", torch.float32, 3)
+    if tuple(weights.shape) != (pages.shape[0], pages.shape[1], KV4_PAGE):
+        raise KernelError(f"token weights are {tuple(weights.shape)}, expected {(pages.shape[0], pages.shape[1], KV4_PAGE)}")
+
+
+@_profiled("kv4_write", lambda out, kv, *a, **k: (_nbytes(kv) + kv.numel() * 9 // 16, 0))
+def kv4_write(kv: torch.Tensor, nkv: int, D: int, *, token_seq, token_pos, slots, block_table, pages, page: int,
+              weights: Optional[torch.Tensor] = None) -> None:
+    """Stores the step's keys and values ``kv`` [T, 2 nkv, D] (keys first; bfloat16 or 32-bit) in a cache of 4 bits
+    (``kv4_pages``): token t at position ``token_pos[t]`` of its sequence's cache.  Every 64 elements x of a key or
+    value become round((x - m) / s) with m their least, rounded down to bfloat16, and s a fifteenth of their range,
+    rounded up; they are read as s c + m, at most s / 2 off.  64 elements of which one is not finite, or whose range
+    bfloat16 does not hold, are read as NaN.  Rows of slot -1 and places outside the block table store nothing; two
+    rows of one call must not have the same place.  ``weights`` (``kv4_weigh``): the new tokens' are set to 0."""
+    _need(kv, "kv rows", ndim=3)
+    a, n, d = _kv4_rows_args(pages, weights, token_seq, token_pos, slots, block_table, page)
+    if (n, d) != (nkv, D) or tuple(kv.shape) != (a.T, 2 * nkv, D):
+        raise KernelError(f"kv rows are {tuple(kv.shape)} for pages of {n} kv heads of {d}, expected [{a.T}, {2 * nkv}, {D}]")
+    if kv.data_ptr() % 16:
+        raise KernelError("kv rows must start on 16 bytes")
+    _same_device(pages, kv)
+    a.kv = kv.data_ptr()
+    f32 = _suffix(kv.dtype) == "f32"
+    with _on(kv):
+        _check(_fn("kv4_cache", "gb_kv4_write", "piip")(ctypes.addressof(a), D, int(f32), _stream()), "kv4_write",
+               1 if a.T else 0)
+
+
+@_profiled("kv4_read", lambda out, pages, **k: (_nbytes(out) + out.numel() * 9 // 16, 0))
+def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, page: int,
+             dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The keys and values [T, 2 nkv, D] that a 4-bit cache holds at the given places, as ``kv4_write`` takes them
+    (``dtype`` bfloat16 or float32: s c + m in 32 bits, rounded once).  Zeros for rows of slot -1 and places outside
+    the block table."""
+    a, nkv, D = _kv4_rows_args(pages, None, token_seq, token_pos, slots, block_table, page)
+    f32 = _suffix(dtype) == "f32"
+    out = torch.empty((a.T, 2 * nkv, D), dtype=dtype, device=pages.device)
+    a.out = out.data_ptr()
+    with _on(pages):
+        _check(_fn("kv4_cache", "gb_kv4_read", "piip")(ctypes.addressof(a), D, int(f32), _stream()), "kv4_read",
+               1 if a.T else 0)
+    return out
+
+
+class _Kv4AttnArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("pages", _P), ("block_table", _P), ("slots", _P), ("kv_len", _P), ("row_seq", _P),
+                ("cu_q", _P), ("out", _P), ("lse", _P), ("part_o", _P), ("part_ml", _P), ("error", _P),
+                ("sinks", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
+                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("n_splits", _I), ("keep_first", _I), ("chunk", _I),
+                ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
+
+
+def kv4_splits(pairs: int, max_kv_len: int, device) -> int:
+    """How many ways the keys of a sequence are split, for ``pairs`` (sequence, group of query heads) pairs."""
+    if DECODE_SPLITS_OVERRIDE:
+        return DECODE_SPLITS_OVERRIDE
+    places = 2 * _sm_count(device)
+    tiles = max(1, (max_kv_len + 63) // 64)
+    most = max(1, min(64, (tiles + 3) // 4))
+    cost = {s: ((pairs * s + places - 1) // places) * (-(-tiles // (4 * s)) + 2.0) for s in range(1, most + 1)}
+    best = min(cost.values())
+    return min(s for s, c in cost.items() if c <= 1.03 * best)
+
+
+def _kv4_query(q, pages, block_table, step, page: int, softcap, window, keep_first, chunk):
+    """The checks that everything shares that takes queries over a 4-bit cache; its sizes."""
+    _need(q, "q", ndim=3)
+    n_pages, nkv, D = _kv4_pages_of(pages)
+    if page != KV4_PAGE:
+        raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
+    if q.shape[2] != D or q.shape[1] % nkv or q.shape[1] == 0:
+        raise KernelError(f"queries are {tuple(q.shape)} for pages of {nkv} kv heads of {D}")
+    if q.data_ptr() % 16:
+        raise KernelError("queries must start on 16 bytes")
+    _need(block_table, "block table", torch.int32, 2)
+    for t, nm in ((step.slots, "slots"), (step.kv_len, "kv_len"), (step.cu_q, "cu_q")):
+        _need(t, nm, torch.int32, 1)
+    n_seqs = step.slots.shape[0]
+    if step.kv_len.shape[0] != n_seqs or step.cu_q.shape[0] != n_seqs + 1:
+        raise KernelError("cu_q, slots and kv_len do not describe one list of sequences")
+    if step.decode and q.shape[0] != n_seqs:
+        raise KernelError(f"{q.shape[0]} rows for {n_seqs} sequences of one token")
+    if (softcap or 0.0) < 0 or (window or 0) < 0 or (keep_first or 0) < 0:
+        raise KernelError("a cap, a window and a number of kept first keys are not negative")
+    _chunk_arg(chunk, keep_first if window else 0)
+    _same_device(q, pages, block_table, step.slots, step.kv_len, step.cu_q)
+    return n_pages, nkv, D
+
+
+def _cost_attention_kv4(out, q, pages, block_table, *, step, window=None, chunk=0, **kw):
+    out = out[0] if isinstance(out, tuple) else out
+    return _attention_cost(out, q, pages.shape[1] * pages.shape[3] // 16, kv_len=step.kv_len, slots=step.slots,
+                           cu_q=step.cu_q, window=window, chunk=chunk)
+
+
+@_profiled("attention_kv4", _cost_attention_kv4)
+def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, *, step, page: int, scale: float,
+                  window: Optional[int] = None, softcap: Optional[float] = None,
+                  sinks: Optional[torch.Tensor] = None, keep_first: int = 0, chunk: int = 0, want_lse: bool = False):
+    """``attention`` over a cache in 4 bits (``kv4_pages``): the step's queries [T, nq, D] over their sequences' cached
+    keys, with the same further terms.  bfloat16 queries take the tensor cores (a step of single tokens with the codes
+    as operands, a prompt with keys and values unpacked to bfloat16), 32-bit queries a 32-bit kernel.  Heads of 64 or
+    128 in groups of any size.  ``want_lse``: (out, lse) with lse [T, nq] 32-bit, the natural logarithm of every
+    softmax's sum (its sink included; -inf for rows of slot -1, whose output is zeros).  A row that would read a page
+    that there is not comes out as NaN; so does one that sees a token stored as NaN (of a value's, at least the 64
+    elements that are)."""
+    T, nq, _D = q.shape if q.dim() == 3 else (0, 0, 0)
+    keep_first = int(keep_first or 0) if window else 0
+    n_pages, nkv, D = _kv4_query(q, pages, block_table, step, page, softcap, window, keep_first, chunk)
+    _check_sinks(sinks, nq)
+    _same_device(q, sinks)
+    f32 = _suffix(q.dtype) == "f32"
+    out = torch.empty_like(q)
+    lse = torch.empty((T, nq), dtype=torch.float32, device=q.device) if want_lse else None
+    if T == 0:
+        return (out, lse) if want_lse else out
+    n_seqs = step.slots.shape[0]
+    if not step.decode and not f32:
+        a = _AttnTcArgs()
+        a.block_table, a.cu_q, a.slots, a.kv_len = (block_table.data_ptr(), step.cu_q.data_ptr(),
+                                                    step.slots.data_ptr(), step.kv_len.data_ptr())
+        a.out, a.error = out.data_ptr(), _tc_error_flag(q.device).data_ptr()
+        a.n_seqs, a.nq, a.nkv, a.max_pages = n_seqs, nq, nkv, block_table.shape[1]
+        a.pack, rows = prefill_tc_plan(lambda n: _q_blocks(step.q_lens, None, n, T, n_seqs), nq, nkv, _sm_count(q.device))
+        a.n_qblocks = _q_blocks(step.q_lens, None, rows // a.pack, T, n_seqs)
+        while a.n_qblocks > 65535 and a.pack > 1:      # more than a grid has: fewer heads, more tokens a block
+            a.pack //= 2
+            a.n_qblocks = _q_blocks(step.q_lens, None, rows // a.pack, T, n_seqs)
+        a.window, a.scale_log2 = int(window or 0), float(scale) * _LOG2E
+        a.keep_first, a.chunk = keep_first, int(chunk or 0)
+        _set_cap_and_sinks(a, scale, softcap, sinks, nq)
+        with _on(q):
+            _check(_fn("attn_prefill_kv4", "gb_attn_prefill_kv4", "ppppiiiiip")(
+                q.data_ptr(), pages.data_ptr(), ctypes.addressof(a), _ptr(lse), T, n_pages, block_table.shape[0], D, rows,
+                _stream()), "attn_prefill_kv4")
+        return (out, lse) if want_lse else out
+    a = _Kv4AttnArgs()
+    if not step.decode:
+        _need(step.token_seq, "token_seq", torch.int32, 1)
+        if step.token_seq.shape[0] != T:
+            raise KernelError(f"token_seq has {step.token_seq.shape[0]} entries for {T} rows")
+        a.row_seq = step.token_seq.data_ptr()
+    per = 4 if f32 else 8
+    groups = nkv * ((nq // nkv + per - 1) // per)
+    ns = kv4_splits((T if f32 else n_seqs) * groups, _keys_visited(step.max_kv_len, window, page, keep_first, int(chunk or 0)),
+                    q.device)
+    if ns > 1:       # (memory of this call's own: two captured graphs, or two streams, share none of it)
+        part = torch.empty(T * nq * ns * (D + 2), dtype=torch.float32, device=q.device)
+        a.part_o, a.part_ml = part.data_ptr(), part[T * nq * ns * D:].data_ptr()
+    a.q, a.pages, a.block_table, a.slots = q.data_ptr(), pages.data_ptr(), block_table.data_ptr(), step.slots.data_ptr()
+    a.kv_len, a.cu_q, a.out, a.lse = step.kv_len.data_ptr(), step.cu_q.data_ptr(), out.data_ptr(), _ptr(lse)
+    a.error = _tc_error_flag(q.device).data_ptr()
+    a.n_rows, a.n_seqs, a.n_slots, a.nq, a.nkv = T, n_seqs, block_table.shape[0], nq, nkv
+    a.max_pages, a.n_pages, a.window, a.n_splits = block_table.shape[1], n_pages, int(window or 0), ns
+    a.keep_first, a.chunk, a.scale_log2 = keep_first, int(chunk or 0), float(scale) * _LOG2E
+    _set_cap_and_sinks(a, scale, softcap, sinks, nq)
+    name = "f32" if f32 else "decode"
+    with _on(q):
+        _check(_fn("attn_kv4", "gb_attn_kv4_" + name, "pip")(ctypes.addressof(a), D, _stream()), "attn_kv4_" + name,
+               2 if ns > 1 else 1)
+    return (out, lse) if want_lse else out
+
+
+class _Kv4WeighArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("lse", _P), ("pages", _P), ("weights", _P), ("block_table", _P), ("slots", _P),
+                ("kv_len", _P), ("cu_q", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
+                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("keep_first", _I), ("chunk", _I), ("last", _I),
+                ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
+
+
+@_profiled("kv4_weigh", lambda out, q, lse, *a, **k: (_nbytes(q, lse), 0))
+def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, *,
+              step, page: int, scale: float, window: Optional[int] = None, softcap: Optional[float] = None,
+              keep_first: int = 0, chunk: int = 0, last: int = 0) -> None:
+    """Adds to every cached token's weight, ``weights`` [pages, kv heads, 64] (32-bit, zeros to begin with), the
+    attention that the step's queries pay it: the sum over the sequence's rows, or its ``last`` ones, and over the kv
+    head's query heads of exp(score - lse), with the queries and the ``lse`` [T, nq] of ``attention_kv4`` and the
+    arguments that it was called with.  (With prompts' lse a weight is exact to the bfloat16 rounding of the keys that
+    they were computed with.)  A sequence must not appear twice in a step."""
+    keep_first = int(keep_first or 0) if window else 0
+    n_pages, nkv, D = _kv4_query(q, pages, block_table, step, page, softcap, window, keep_first, chunk)
+    if q.dtype != torch.bfloat16:
+        raise KernelError(f"weights are gathered from bfloat16 queries, not {q.dtype}")
+    T, nq, _D = q.shape
+    _need(lse, "lse", torch.float32, 2)
+    if tuple(lse.shape) != (T, nq):
+        raise KernelError(f"lse is {tuple(lse.shape)}, expected {(T, nq)}")
+    _check_kv4_weights(weights, pages)
+    _same_device(q, lse, weights)
+    if int(last) < 0:
+        raise KernelError("the number of last rows is not negative")
+    a = _Kv4WeighArgs()
+    a.q, a.lse, a.pages, a.weights = q.data_ptr(), lse.data_ptr(), pages.data_ptr(), weights.data_ptr()
+    a.block_table, a.slots = block_table.data_ptr(), step.slots.data_ptr()
+    a.kv_len, a.cu_q = step.kv_len.data_ptr(), step.cu_q.data_ptr()
+    a.n_rows, a.n_seqs, a.n_slots, a.nq, a.nkv = T, step.slots.shape[0], block_table.shape[0], nq, nkv
+    a.max_pages, a.n_pages, a.window, a.last = block_table.shape[1], n_pages, int(window or 0), int(last)
+    a.keep_first, a.chunk, a.scale_log2 = keep_first, int(chunk or 0), float(scale) * _LOG2E
+    a.cap_log2 = float(softcap) * _LOG2E if softcap else 0.0
+    a.cap_inv = float(scale) / float(softcap) if softcap else 0.0
+    blocks = max(1, (step.max_kv_len + KV4_PAGE - 1) // KV4_PAGE)
+    with _on(q):
+        _check(_fn("attn_kv4", "gb_kv4_weigh", "piip")(ctypes.addressof(a), D, min(blocks, 65535), _stream()), "kv4_weigh",
+               1 if T else 0)
+
+
+class _Kv4ChooseArgs(ctypes.Structure):
+    _fields_ = [("weights", _P), ("block_table", _P), ("slots", _P), ("kv_len", _P), ("kept", _P), ("new_len", _P),
+                ("n_seqs", _I), ("n_slots", _I), ("nkv", _I), ("max_pages", _I), ("n_pages", _I), ("keep", _I),
+                ("recent", _I), ("first", _I)]
+
+
+class _Kv4MoveArgs(ctypes.Structure):
+    _fields_ = [("src", _P), ("to", _P), ("w_src", _P), ("w_to", _P), ("src_table", _P), ("to_table", _P),
+                ("slots", _P), ("kept", _P), ("n_seqs", _I), ("n_slots", _I), ("nkv", _I), ("n_pages", _I), ("keep", _I),
+                ("src_max", _I), ("to_max", _I), ("in_order", _I)]
+
+
+@_profiled("kv4_evict", lambda out, pages, *a, **k: (2 * out[0].numel() * (pages.shape[3] // 16 + 4), 0))
+def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, *, slots: torch.Tensor,
+              kv_len: torch.Tensor, page: int, keep: int, recent: int, first: int = 0,
+              into: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cuts sequences of more than ``keep`` tokens to ``keep``: every kv head keeps the sequence's ``first`` tokens, its
+    ``recent`` newest, and of the others those with the largest ``weights`` (``kv4_weigh``; the earlier of equal ones, a
+    NaN above everything).  The kept tokens move to places 0 .. keep - 1 in the order in which they stood, with their
+    weights; keys are not turned again, so a sequence's next token keeps its own position and goes to place ``keep``.
+    Returns (kept int32 [sequences, kv heads, keep]: the places that they stood at, -1 behind the last; the new lengths
+    int32 [sequences]).  Sequences of slot -1 keep nothing, shorter ones all they have.  ``into``: a block table like
+    ``block_table`` whose pages take the kept tokens (pages that no sequence of the call reads from); without it they
+    stay in the sequence's first pages.  A slot must not appear twice."""
+    n_pages, nkv, D = _kv4_pages_of(pages)
+    if page != KV4_PAGE:
+        raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
+    _check_kv4_weights(weights, pages)
+    _need(block_table, "block table", torch.int32, 2)
+    for t, nm in ((slots, "slots"), (kv_len, "kv_len")):
+        _need(t, nm, torch.int32, 1)
+    n_seqs, keep, recent, first = slots.shape[0], int(keep), int(recent), int(first)
+    if kv_len.shape[0] != n_seqs:
+        raise KernelError(f"{n_seqs} slots with {kv_len.shape[0]} lengths")
+    if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
+        raise KernelError(f"{first} first and {recent} recent tokens do not fit {keep} that are kept")
+    if into is not None:
+        _need(into, "block table of the kept tokens", torch.int32, 2)
+        if into.shape[0] != block_table.shape[0] or into.shape[1] * KV4_PAGE < min(keep, block_table.shape[1] * KV4_PAGE):
+            raise KernelError(f"the block table of the kept tokens is {tuple(into.shape)} for {keep} tokens of "
+                              f"{block_table.shape[0]} slots")
+    _same_device(pages, weights, block_table, slots, kv_len, into)
+    kept = torch.empty((n_seqs, nkv, keep), dtype=torch.int32, device=pages.device)
+    lens = torch.empty((n_seqs,), dtype=torch.int32, device=pages.device)
+    if n_seqs == 0:
+        return kept, lens
+    c = _Kv4ChooseArgs()
+    c.weights, c.block_table, c.slots, c.kv_len = weights.data_ptr(), block_table.data_ptr(), slots.data_ptr(), kv_len.data_ptr()
+    c.kept, c.new_len, c.n_seqs, c.n_slots, c.nkv = kept.data_ptr(), lens.data_ptr(), n_seqs, block_table.shape[0], nkv
+    c.max_pages, c.n_pages, c.keep, c.recent, c.first = block_table.shape[1], n_pages, keep, recent, first
+    m = _Kv4MoveArgs()
+    m.slots, m.kept, m.n_seqs, m.n_slots, m.nkv, m.n_pages, m.keep = (slots.data_ptr(), kept.data_ptr(), n_seqs,
+                                                                     block_table.shape[0], nkv, n_pages, keep)
+    m.src, m.w_src, m.src_table, m.src_max = pages.data_ptr(), weights.data_ptr(), block_table.data_ptr(), block_table.shape[1]
+    m.to, m.w_to = pages.data_ptr(), weights.data_ptr()
+    in_place = into is None or into.data_ptr() == block_table.data_ptr()
+    with _on(pages):
+        _check(_fn("kv4_cache", "gb_kv4_choose", "pp")(ctypes.addressof(c), _stream()), "kv4_choose")
+        move = _fn("kv4_cache", "gb_kv4_move", "pip")
+        if in_place:      # by way of memory of this call's own: tokens move within the pages that others are read from
+            records = (keep + 15) // 16
+            held = torch.empty((n_seqs, nkv, records, pages.shape[3]), dtype=torch.uint8, device=pages.device)
+            w_held = torch.empty((n_seqs, nkv, records * 16), dtype=torch.float32, device=pages.device)
+            m.to, m.w_to, m.to_table = held.data_ptr(), w_held.data_ptr(), None
+            _check(move(ctypes.addressof(m), D, _stream()), "kv4_move")
+            m.src, m.w_src, m.src_table, m.in_order = held.data_ptr(), w_held.data_ptr(), None, 1
+            m.to, m.w_to = pages.data_ptr(), weights.data_ptr()
+            m.to_table, m.to_max = block_table.data_ptr(), block_table.shape[1]
+        else:
+            m.to_table, m.to_max = into.data_ptr(), into.shape[1]
+        _check(move(ctypes.addressof(m), D, _stream()), "kv4_move")
+    return kept, lens
 
 
 # ---------------------------------------------------------------- differential attention
