@@ -1,6 +1,8 @@
 // Attention of single tokens over the cache in 4 bits (kv4.cuh), in bfloat16 on the tensor cores and in 32 bits, and
 // the weights that the cached tokens gather from it.
-#include "attn_mma.cuh"   // ScoreCap, add_sink, mma_16816
+#include <cuda_fp16.h>
+
+#include "attn_mma.cuh"   // ScoreCap, add_sink
 #include "kv4.cuh"
 #include "tc_common.cuh"  // mbarriers with bounded waits
 
@@ -18,9 +20,12 @@ struct Kv4AttnArgs {
   float* lse;              // [rows, nq] or null
   float* part_o;           // [rows, nq, n_splits, D]   (n_splits > 1)
   float* part_ml;          // [rows, nq, n_splits, 2]
+  int* pieces;             // [rows, nkv * groups of heads]: how many splits a row has (n_splits > 1)
   int* error;
   const float* sinks;      // [nq] one more logit of every head's denominator, or null
   int n_rows, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window, n_splits;
+  int per;                 // stretches of 32 keys of a split; shared out: that a block takes at least
+  int shared;              // the blocks share the stretches out evenly
   int keep_first, chunk;
   float scale_log2;
   ScoreCap cap;
@@ -46,71 +51,202 @@ struct Stretches {
   __device__ __forceinline__ int at(int v) const { return v < n_kept ? v : first + v - n_kept; }
 };
 
+// The position of row t among its sequence's keys (-1 with no keys), and whether the row is of a sequence at all.
+__device__ __forceinline__ bool find_row(const Kv4AttnArgs& a, int t, int& pos) {
+  const int seq = a.row_seq ? a.row_seq[t] : t;
+  pos = -1;
+  if ((unsigned)seq >= (unsigned)a.n_seqs || (unsigned)a.slots[seq] >= (unsigned)a.n_slots) return false;
+  pos = a.kv_len[seq] - 1 - (a.row_seq ? a.cu_q[seq + 1] - 1 - t : 0);
+  pos = min(pos, a.max_pages * KV4_PAGE);             // (the first place that there is not: it makes the row NaN)
+  return true;
+}
+
 // ---------------------------------------------------------------- bfloat16, single tokens
+#define KV4_SHARED_SEQS 256      // the most sequences whose stretches are shared out (their counts lie beside four rings an SM)
+
+// before[i]: the stretches of the sequences in front of i (of one pair of each).  Returns how many stretches a block
+// takes.  For a whole block of 128 threads.
+__device__ __forceinline__ unsigned share_out(const Kv4AttnArgs& a, int unit, int groups, int* before) {
+  __shared__ int warp_sums[4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (a.n_seqs + 127) / 128;
+  int mine = 0;
+  for (int i = tid * each; i < min(a.n_seqs, (tid + 1) * each); ++i) {
+    int pos;
+    find_row(a, i, pos);
+    mine += Stretches(pos, unit, a.window, a.keep_first, a.chunk).n;
+  }
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int below = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += below;
+  }
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w == warp) sum += all;
+    all += warp_sums[w];
+  }
+  int here = sum - mine;
+  for (int i = tid * each; i < min(a.n_seqs, (tid + 1) * each); ++i) {
+    int pos;
+    find_row(a, i, pos);
+    before[i] = here;
+    here += Stretches(pos, unit, a.window, a.keep_first, a.chunk).n;
+  }
+  if (tid == 0) before[a.n_seqs] = all;
+  __syncthreads();
+  return max((unsigned)a.per, ((unsigned)all * groups + gridDim.x - 1) / gridDim.x);
+}
+
+// The sequence that stretch x (of one pair of each sequence) belongs to: the last with before <= x that has any.
+__device__ __forceinline__ int find_stretch(const int* before, int n_seqs, unsigned x) {
+  int lo = 0, hi = n_seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if ((unsigned)before[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The row of a sequence without keys: zeros (its sink has all the weight, where there is one).
+__device__ __forceinline__ void empty_row(const Kv4AttnArgs& a, int seq, int groups, int D) {
+  int pos;
+  const bool live = find_row(a, seq, pos);
+  for (int i = threadIdx.x; i < a.nq * D; i += blockDim.x) reinterpret_cast<bf16*>(a.out)[(size_t)seq * a.nq * D + i] = __float2bfloat16(0.f);
+  if (a.lse)
+    for (int i = threadIdx.x; i < a.nq; i += blockDim.x)
+      a.lse[(size_t)seq * a.nq + i] = live && a.sinks ? a.sinks[i] : -INFINITY;
+  for (int i = threadIdx.x; i < groups; i += blockDim.x) a.pieces[(size_t)seq * groups + i] = 1;
+}
+
 template <int D>
 struct Kv4Decode {
   static constexpr int WARPS = 4;
-  static constexpr int STAGES = 3;
-  static constexpr int UNIT = 64;                               // keys of a stage: whole records of one page
+  static constexpr int STAGES = 2;
+  static constexpr int UNIT = 32;                               // keys of a stage: whole records of one page
   static constexpr int RECORDS = UNIT / KV4_TOKENS;
   static constexpr int STAGE_BYTES = RECORDS * Kv4<D>::RECORD;
   static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
-  static constexpr int MERGE = WARPS * 8 * (D + 2) * 4;         // the warps' results, where the ring was
-  static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + 128;
+  // The warps' results: 8 heads each, a head's elements in the order (word's element, lane group) under a pitch that
+  // puts a store's 32 lanes into 32 banks.
+  static constexpr int PITCH = D + 4;
+  static constexpr int MERGE = WARPS * 8 * (PITCH + 2) * 4;
+  static constexpr int SMEM = RING + MERGE + 128;
+};
+
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+
+// The eight codes of a word less 8, as four registers of two half-precision numbers (elements 2 i and 2 i + 1; exact).
+// A nibble in the low bits of 1024's mantissa is 1024 + c, in the next four 1024 + 16 c, so that a word takes one shift
+// and four logical operations, and the multiply-adds that take the rest off run beside them in the other pipe.  (The
+// logical pipe has half the rate and bounds these kernels: as bfloat16 numbers, 1 + c / 16, a word takes eight of it.)
+// `magic` is 1024 in both halves, from kv4_magic(): an instruction takes one constant, and with two of them the compiler
+// makes two instructions of every one of these (144 of them a record instead of 72).
+#define KV4_1024 0x64006400u
+__device__ __forceinline__ uint32_t kv4_magic(int not_negative) { return KV4_1024 ^ (uint32_t)(not_negative >> 31); }
+template <uint32_t MASK>
+__device__ __forceinline__ __half2 kv4_nibbles(uint32_t w, uint32_t magic) {
+  uint32_t x;                                          // (w & MASK) | magic
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(MASK), "r"(magic));
+  return as_half2(x);
+}
+__device__ __forceinline__ void kv4_codes(uint32_t w, uint32_t magic, uint32_t (&x)[4]) {
+  const __half2 low = __floats2half2_rn(-1032.f, -1032.f), high = __floats2half2_rn(-72.f, -72.f);
+  const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+  const uint32_t v = w >> 8;
+  x[0] = as_u32(__hadd2(kv4_nibbles<0x000f000fu>(w, magic), low));
+  x[1] = as_u32(__hfma2(kv4_nibbles<0x00f000f0u>(w, magic), sixteenth, high));
+  x[2] = as_u32(__hadd2(kv4_nibbles<0x000f000fu>(v, magic), low));
+  x[3] = as_u32(__hfma2(kv4_nibbles<0x00f000f0u>(v, magic), sixteenth, high));
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight query heads as the B operand of the scores: this lane's part of head lane / 4 (words n with n % 4 = lane % 4 of
+// its row) in half precision, divided by a power of two that brings the head's largest element into [1, 2): a bfloat16
+// element then loses nothing, but for those 2^-15 of the largest and below, which keep 2^-25 of it.  Of heads 2 t and
+// 2 t + 1: the sums over the groups (divided too) and the power of two.
+template <int D>
+struct Kv4Query {
+  uint32_t q[D / 32][4];
+  float sum[D / 64][2], back[2];
+  __device__ __forceinline__ void load(const bf16* row) {       // null: zeros
+    const int t = threadIdx.x & 3;
+    float x[D / 32][8], top = 0.f;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row) v = *reinterpret_cast<const uint4*>(row + 8 * (4 * w + t));
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[w][2 * i] = __uint_as_float(u[i] << 16), x[w][2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        top = fmaxf(top, fmaxf(fabsf(x[w][2 * i]), fabsf(x[w][2 * i + 1])));
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e <= top, within what a float's inverse can be
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+    const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+    float part[D / 64];
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) part[g] = 0.f;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(x[w][2 * i] * down, x[w][2 * i + 1] * down);
+        q[w][i] = as_u32(h);
+        part[w / 2] += x[w][2 * i] * down + x[w][2 * i + 1] * down;
+      }
+#pragma unroll
+    for (int g = 0; g < D / 64; ++g) {
+      float s = part[g];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      sum[g][0] = __shfl_sync(0xffffffffu, s, 8 * t);           // head 2 t lies in lanes 4 (2 t) ...
+      sum[g][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+    }
+    back[0] = __shfl_sync(0xffffffffu, up, 8 * t);
+    back[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+  }
 };
 
 // The scores of a record's 16 tokens with eight query heads: s[0], s[1] are row r's with heads 2 t, 2 t + 1, s[2], s[3]
-// row r + 8's, in units of q . k.  The products see a code c as 1 + c / 16; they start from minus the sum of the
-// query's elements, so that they end as the sum of q c / 16, and a group's pair then makes 16 s of it and adds m times
-// the query's sum.  (Everything is exact but the 32-bit sums: a bfloat16 query times five bits.)
+// row r + 8's, in units of q . k over the heads' powers of two.  Products of a half-precision query and codes less 8
+// are exact, their sums 32-bit; a group's pair makes s of them and adds m + 8 s times the query's sum.
 template <int D>
 __device__ __forceinline__ void kv4_scores(const uint32_t (&ka)[D / 32], const uint32_t (&kb)[D / 32], const uint32_t* pa,
-                                           const uint32_t* pb, const uint32_t (&q)[D / 32][4],
-                                           const float (&qsum)[D / 64][2], float (&s)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = 0.f;
+                                           const uint32_t* pb, const Kv4Query<D>& q, uint32_t magic, float (&s)[4]) {
 #pragma unroll
   for (int g = 0; g < D / 64; ++g) {
-    float acc[4] = {-qsum[g][0], -qsum[g][1], -qsum[g][0], -qsum[g][1]};
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 2 * g; w < 2 * g + 2; ++w) {
-      const uint32_t a0[4] = {kv4_two<0>(ka[w]), kv4_two<0>(kb[w]), kv4_two<1>(ka[w]), kv4_two<1>(kb[w])};
-      mma_16816(acc, a0, q[w][0], q[w][1]);
-      const uint32_t a1[4] = {kv4_two<2>(ka[w]), kv4_two<2>(kb[w]), kv4_two<3>(ka[w]), kv4_two<3>(kb[w])};
-      mma_16816(acc, a1, q[w][2], q[w][3]);
+      uint32_t xa[4], xb[4];
+      kv4_codes(ka[w], magic, xa);
+      kv4_codes(kb[w], magic, xb);
+      mma_f16(acc, xa[0], xb[0], xa[1], xb[1], q.q[w][0], q.q[w][1]);
+      mma_f16(acc, xa[2], xb[2], xa[3], xb[3], q.q[w][2], q.q[w][3]);
     }
-    const float sa = 16.f * kv4_s(pa[g]), ma = kv4_m(pa[g]), sb = 16.f * kv4_s(pb[g]), mb = kv4_m(pb[g]);
-    s[0] += fmaf(sa, acc[0], ma * qsum[g][0]);
-    s[1] += fmaf(sa, acc[1], ma * qsum[g][1]);
-    s[2] += fmaf(sb, acc[2], mb * qsum[g][0]);
-    s[3] += fmaf(sb, acc[3], mb * qsum[g][1]);
-  }
-}
-
-// This lane's part of eight query heads as the B operand (head lane / 4; words n with n % 4 = lane % 4 of its row) and
-// the sums of heads 2 t, 2 t + 1 over the groups.  `row`: the head's D elements, or null (zeros).
-template <int D>
-__device__ __forceinline__ void kv4_query(const bf16* row, uint32_t (&q)[D / 32][4], float (&qsum)[D / 64][2]) {
-  const int lane = threadIdx.x & 31, t = lane & 3;
-  float part[D / 64];
+    const float sa = kv4_s(pa[g]), ma = fmaf(8.f, sa, kv4_m(pa[g])), sb = kv4_s(pb[g]), mb = fmaf(8.f, sb, kv4_m(pb[g]));
 #pragma unroll
-  for (int g = 0; g < D / 64; ++g) part[g] = 0.f;
-#pragma unroll
-  for (int w = 0; w < D / 32; ++w) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row) v = *reinterpret_cast<const uint4*>(row + 8 * (4 * w + t));
-    q[w][0] = v.x, q[w][1] = v.y, q[w][2] = v.z, q[w][3] = v.w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      part[w / 2] += __uint_as_float(q[w][i] << 16) + __uint_as_float(q[w][i] & 0xffff0000u);
-  }
-#pragma unroll
-  for (int g = 0; g < D / 64; ++g) {
-    float x = part[g];
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    x += __shfl_xor_sync(0xffffffffu, x, 2);
-    qsum[g][0] = __shfl_sync(0xffffffffu, x, 8 * t);        // head 2 t lies in lanes 4 (2 t) ...
-    qsum[g][1] = __shfl_sync(0xffffffffu, x, 8 * t + 4);
+    for (int i = 0; i < 4; ++i) {
+      const float m = i < 2 ? ma : mb, x = i < 2 ? sa : sb;
+      s[i] = g == 0 ? m * q.sum[g][i & 1] : fmaf(m, q.sum[g][i & 1], s[i]);
+      s[i] = fmaf(x, acc[i], s[i]);
+    }
   }
 }
 
@@ -140,271 +276,417 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Block (split, group of up to eight query heads of one kv head, sequence); every warp takes stretches of 64 keys in
-// turn, each through a ring of its own that bulk copies fill, and keeps its own maximum, sum and accumulator: no
-// barrier of the block lies in the loop.  For 16 tokens at a time
+// The blocks share out the stretches of 32 keys of all pairs (sequence, group of up to eight query heads of one kv head)
+// evenly, in the order of the pairs: a block has one run of them, which may end inside a pair and go on in the next, so
+// sequences of unequal lengths leave no SM waiting (60 sequences of 700 to 4,096 keys: SPLIT_US us with a fixed number of
+// keys a block, which the SMs were through with between 59 and 105 thousand cycles, SHARED_US so).  With one split a
+// block has a whole pair.
+// Of a run's part of a pair every warp takes stretches in turn, each through a ring of its own that bulk copies fill,
+// and keeps its own maximum, sum and accumulator: no barrier of the block lies in the loop.  For the two records of a
+// stretch
 //   S = K q^T       m16n8k16 products, rows tokens, columns heads (kv4_scores)
 //   P = 2^(S c - m) in registers; times the value's s it becomes the B operand of the second product by a transposition
 //                   of 8 x 8 numbers among the lanes
 //   O += V^T P      rows the head's elements, columns heads
-// so the codes go from shared memory straight into operands: a word of them is a load, and a shift and a logical
-// operation for every two elements.  Values are seen as 1 + c / 16 too: O's excess is the sum of the rounded P, which
-// one more product with ones keeps in step, so nothing is lost to the rounding of P.
-template <int D>
-__global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32) kv4_decode_kernel(const Kv4AttnArgs a) {
+// so the codes go from shared memory straight into operands.  P s is half-precision: it is divided by a power of two
+// near the largest s that the warp has met (raised when an s is 2^6 beyond it), and the base of the exponents keeps P
+// below 2^8, so it stays below 2^15 and what it loses at the other end is below 2^-25 of a whole probability.  Values
+// are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range; m + 8 s times P
+// is summed in 32 bits.
+// A block's part of a pair, for all its threads.
+struct Kv4Part {
+  int seq, group, piece, n_pieces;
+};
+
+// BOUNDED: there is a window or chunks, so the list of stretches may have a gap and a first key.
+template <int D, bool BOUNDED>
+__global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel(const Kv4AttnArgs a) {
   using F = Kv4<D>;
   using C = Kv4Decode<D>;
-  constexpr int NG = F::NG;
+  constexpr int NG = F::NG, NR = C::RECORDS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[C::WARPS][C::STAGES];
+  __shared__ int before[KV4_SHARED_SEQS + 1];
+  __shared__ Kv4Part part_s[2];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int r = lane >> 2, t = lane & 3;
   const int G = a.nq / a.nkv, hgroups = (G + 7) / 8;
-  const int split = blockIdx.x, kvh = blockIdx.y / hgroups, hg = blockIdx.y % hgroups, seq = blockIdx.z;
-  const int h0 = kvh * G + hg * 8, heads = min(8, G - hg * 8);
+  const int groups = a.nkv * hgroups;
   if (lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[warp][s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
   pdl_wait();
-  const int slot = a.slots[seq];
-  const bool live = (unsigned)slot < (unsigned)a.n_slots;
-  const int pos = live ? a.kv_len[seq] - 1 : -1;
-  const Stretches list(pos, C::UNIT, a.window, a.keep_first, a.chunk);
   const int keep = a.window > 0 ? a.keep_first : 0;
-  const int per = (list.n + a.n_splits - 1) / a.n_splits;
-  const int v_end = min(list.n, (split + 1) * per), v0 = split * per + warp;
-  const int* table = a.block_table + (size_t)(live ? slot : 0) * a.max_pages;
   uint8_t* ring = smem + warp * C::STAGES * C::STAGE_BYTES;
+  const uint32_t magic = kv4_magic(a.n_seqs);
+  uint32_t parity = 0;                               // the phases to wait for, by stage
+  bool ok = true;
 
-  // asks for stretch v (a whole warp calls; one lane asks): true when something comes
+  // this block's run [at, end) of the list of all stretches; before[i]: those of one pair of each sequence in front of i
+  unsigned at = 0, end = 0, run = 1;
+  int seq_next = blockIdx.x / (groups * a.n_splits);
+  bool more = true;
+  if (a.shared) {
+    run = share_out(a, C::UNIT, groups, before);
+    at = run * blockIdx.x;
+    end = min(at + run, (unsigned)before[a.n_seqs] * groups);
+    for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x)      // sequences without keys have nobody else
+      if (before[i + 1] == before[i]) empty_row(a, i, groups, D);
+    seq_next = find_stretch(before, a.n_seqs, at / groups);
+    more = at < end;
+  }
+  if (!more) return;
+
+  // The part that is worked on: its sequence's last position and first key, its stretches [v, v_end) of this warp, what
+  // is on its way.  begin() finds the block's next part and asks for its first stretches; the results of the part
+  // before are put together while they come.
+  int pos = 0, lo = 0, v = 0, v_end = 0, gap_at = 0, gap = 0, page_next = 0;
+  const int* table = nullptr;
+  const uint8_t* head = nullptr;                     // the kv head's records of page 0
+  uint32_t asked = 0;                                // stages with something on its way
   bool lost = false;                                 // a page that there is not: the result is NaN
-  auto ask = [&](int v, int stage) {
-    const int key0 = list.at(v) * C::UNIT;
-    const int page = kv4_page(table, key0 / KV4_PAGE, a.max_pages, a.n_pages);
+  const size_t page_bytes = (size_t)a.nkv * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
+  auto first_of = [&](int u) { return (BOUNDED && u >= gap_at ? u + gap : u) * C::UNIT; };
+  // The page of a stretch is looked up a turn before the stretch is asked for: the answer takes hundreds of cycles, in
+  // which a warp that needs it does nothing else.
+  auto page_of = [&](int u) {
+    return u < v_end ? kv4_page(table, first_of(u) / KV4_PAGE, a.max_pages, a.n_pages) : 0;
+  };
+  // asks for stretch u (a whole warp calls; one lane asks): true when something comes
+  auto ask = [&](int u, int page, int stage) {
     if (page < 0) {
       lost = true;
       return false;
     }
-    const int records = min(C::RECORDS, (pos - key0) / KV4_TOKENS + 1);
     if (elect_one()) {
-      const uint32_t bytes = records * F::RECORD;
+      const int key0 = first_of(u);
+      const uint32_t bytes = min(NR, (pos - key0) / KV4_TOKENS + 1) * F::RECORD;
       mbar_expect_tx(&full[warp][stage], bytes);
-      bulk_load(ring + stage * C::STAGE_BYTES,
-                a.pages + (((size_t)page * a.nkv + kvh) * (KV4_PAGE / KV4_TOKENS) + (key0 % KV4_PAGE) / KV4_TOKENS) * F::RECORD,
-                bytes, &full[warp][stage]);
+      bulk_load(ring + stage * C::STAGE_BYTES, head + page * page_bytes + key0 % KV4_PAGE / KV4_TOKENS * F::RECORD, bytes,
+                &full[warp][stage]);
     }
     __syncwarp();
     return true;
   };
-  uint32_t asked = 0, parity = 0;                    // stages with something on its way; the phase to wait for
-#pragma unroll
-  for (int s = 0; s < C::STAGES; ++s)
-    if (v0 + s * C::WARPS < v_end && ask(v0 + s * C::WARPS, s)) asked |= 1u << s;
-
-  uint32_t q[D / 32][4];
-  float qsum[NG][2];
-  kv4_query<D>(r < heads ? reinterpret_cast<const bf16*>(a.q) + ((size_t)seq * a.nq + h0 + r) * D : nullptr, q, qsum);
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // of heads 2 t, 2 t + 1; l and off: this lane's rows only
-  float o[NG][4][4], ones_o[NG][4], off[NG][2];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    off[g][0] = off[g][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ones_o[g][i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[g][i][c] = 0.f;
+  int turn_of = 0;                                   // which of part_s has the part that is worked on
+  auto begin = [&]() {
+    Kv4Part part;
+    part.seq = seq_next;
+    const bool live = find_row(a, part.seq, pos);
+    const int slot = live ? a.slots[part.seq] : 0;
+    const Stretches list(pos, C::UNIT, BOUNDED ? a.window : 0, BOUNDED ? a.keep_first : 0, BOUNDED ? a.chunk : 0);
+    int v_begin;
+    if (a.shared) {
+      const unsigned first = (unsigned)before[part.seq] * groups, n = (unsigned)list.n;
+      part.group = (int)((at - first) / n);
+      const unsigned pair = first + part.group * n, piece0 = pair / run;
+      v_begin = (int)(at - pair);
+      v_end = (int)min(n, v_begin + (end - at));
+      part.piece = (int)(blockIdx.x - piece0);
+      part.n_pieces = (int)((pair + n - 1) / run - piece0) + 1;
+      at += v_end - v_begin;
+      more = at < end;
+      if (at == (unsigned)before[part.seq + 1] * groups && more)
+        do ++seq_next; while (before[seq_next + 1] == before[seq_next]);      // (there is one with keys)
+    } else {
+      part.group = blockIdx.x / a.n_splits % groups, part.piece = blockIdx.x % a.n_splits;
+      part.n_pieces = a.n_splits > 1 ? (list.n + a.per - 1) / a.per : 1;
+      v_begin = part.piece * a.per;
+      v_end = a.n_splits > 1 ? min(list.n, v_begin + a.per) : list.n;
+      more = false;
     }
-  }
-  const bool capped = a.cap.cap_log2 != 0.f;
-  const int tok_a = kv4_token(r), k_tok = t, k_tok1 = 4 + (t ^ 1);   // tokens of this lane's rows, of its columns
-  const int v_word = (r ^ ((t & 2) << 1)) * NG;
-  bool ok = true;
+    if (threadIdx.x == 0) part_s[turn_of] = part;
+    v = v_begin + warp;
+    lo = list.lo, gap_at = list.n_kept, gap = list.first - list.n_kept;
+    table = a.block_table + (size_t)slot * a.max_pages;
+    head = a.pages + (size_t)(part.group / hgroups) * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
+    lost = false;
+    asked = 0;
+    int page[C::STAGES + 1];
+#pragma unroll
+    for (int s = 0; s <= C::STAGES; ++s) page[s] = page_of(v + s * C::WARPS);
+#pragma unroll
+    for (int s = 0; s < C::STAGES; ++s)
+      if (ok && v + s * C::WARPS < v_end && ask(v + s * C::WARPS, page[s], s)) asked |= 1u << s;
+    page_next = page[C::STAGES];
+    return part;
+  };
 
-  int stage = 0;
-  for (int v = v0; v < v_end; v += C::WARPS) {
-    if (asked >> stage & 1) {
-      if (!mbar_wait_warp(&full[warp][stage], parity >> stage & 1, nullptr)) { ok = false; break; }
-      parity ^= 1u << stage;
-      const uint8_t* unit = ring + stage * C::STAGE_BYTES;
-      const int key0 = list.at(v) * C::UNIT;
-      const int records = min(C::RECORDS, (pos - key0) / KV4_TOKENS + 1);
-      const bool edge = key0 < list.lo || key0 + C::UNIT - 1 > pos;
+  const int tok_a = kv4_token(r), k_tok = t, k_tok1 = 4 + (t ^ 1);   // tokens of this lane's rows, of its columns
+  const int k_at = tok_a * F::ROW + t * (D / 8), p_at = F::PAIR_OFF + tok_a * F::PAIR;
+  const int v_word = (r ^ ((t & 2) << 1)) * NG;
+  const int v_at = F::V_OFF + k_tok * F::ROW + v_word * 4, v_at1 = F::V_OFF + k_tok1 * F::ROW + v_word * 4;
+  const bool capped = a.cap.cap_log2 != 0.f;
+  float* red_o = reinterpret_cast<float*>(smem + C::RING);     // [warps][8][PITCH]
+  float* red_ml = red_o + C::WARPS * 8 * C::PITCH;             // [warps][8][2]
+
+  Kv4Part part = begin();
+  if (part.piece > 0 && part.piece >= part.n_pieces) return;   // (a split without keys: nothing has been asked for)
+  for (;;) {
+    Kv4Query<D> q;
+    {
+      const int h = part.group % hgroups * 8 + r;
+      q.load(h < G ? reinterpret_cast<const bf16*>(a.q) + ((size_t)part.seq * a.nq + part.group / hgroups * G + h) * D : nullptr);
+    }
+    const float unit_scale = capped ? a.cap.cap_inv : a.scale_log2;
+    const float factor[2] = {unit_scale * q.back[0], unit_scale * q.back[1]};
+
+    // of heads 2 t, 2 t + 1: the base of the exponents, the base or 0 where there is none, the base and 2^8; the sum of
+    // P and of P (m + 8 s) over this lane's rows
+    float m[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f}, most[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[NG][4][4], off[NG][2];
+    float s_most = 0.f, s_down = 1.f;                // an s beyond the first raises the power of two; its inverse
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      off[g][0] = off[g][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[g][i][c] = 0.f;
+    }
+
+    int stage = 0;
 #pragma unroll 1
-      for (int rec = 0; rec < records; ++rec) {
-        const uint8_t* b = unit + rec * F::RECORD;
-        uint32_t ka[D / 32], kb[D / 32], pa[2 * NG], pb[2 * NG];
-        load_words(b + tok_a * F::ROW + t * (D / 8), ka);
-        load_words(b + (tok_a + 8) * F::ROW + t * (D / 8), kb);
-        load_words(b + F::PAIR_OFF + tok_a * F::PAIR, pa);
-        load_words(b + F::PAIR_OFF + (tok_a + 8) * F::PAIR, pb);
-        uint32_t va[4][NG];
-        load_words(b + F::V_OFF + k_tok * F::ROW + v_word * 4, va[0]);
-        load_words(b + F::V_OFF + k_tok1 * F::ROW + v_word * 4, va[1]);
-        load_words(b + F::V_OFF + (k_tok + 8) * F::ROW + v_word * 4, va[2]);
-        load_words(b + F::V_OFF + (k_tok1 + 8) * F::ROW + v_word * 4, va[3]);
-        float s[4];
-        kv4_scores<D>(ka, kb, pa, pb, q, qsum, s);
+    for (; v < v_end && ok; v += C::WARPS) {
+      const int page_now = page_next;
+      page_next = page_of(v + (C::STAGES + 1) * C::WARPS);
+      if (asked >> stage & 1) {
+        if (!mbar_wait_warp(&full[warp][stage], parity >> stage & 1, nullptr)) { ok = false; break; }
+        parity ^= 1u << stage;
+        const uint8_t* unit = ring + stage * C::STAGE_BYTES;
+        const int key0 = first_of(v);
+        float s[NR][4];
+        uint32_t vp[NR][2][NG];                      // the values' pairs of this lane's two rows
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+          const uint8_t* b = unit + u * F::RECORD;
+          uint32_t ka[D / 32], kb[D / 32], pa[2 * NG], pb[2 * NG];
+          load_words(b + k_at, ka);
+          load_words(b + k_at + 8 * F::ROW, kb);
+          load_words(b + p_at, pa);
+          load_words(b + p_at + 8 * F::PAIR, pb);
+          kv4_scores<D>(ka, kb, pa, pb, q, magic, s[u]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) vp[u][0][g] = pa[NG + g], vp[u][1][g] = pb[NG + g];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][i] *= factor[i & 1];
+        }
         if (capped) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[i] = capped_log2(s[i] * a.cap.cap_inv, a.cap);
-        } else {
+          for (int u = 0; u < NR; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[i] *= a.scale_log2;
+            for (int i = 0; i < 4; ++i) s[u][i] = capped_log2(s[u][i], a.cap);
         }
-        bool see_a = true, see_b = true;
-        if (edge) {
-          const int ja = key0 + rec * KV4_TOKENS + tok_a, jb = ja + 8;
-          see_a = ja <= pos && (ja >= list.lo || ja < keep);
-          see_b = jb <= pos && (jb >= list.lo || jb < keep);
-          if (!see_a) s[0] = s[1] = -INFINITY;
-          if (!see_b) s[2] = s[3] = -INFINITY;
+        if ((BOUNDED && key0 < lo) || key0 + C::UNIT - 1 > pos) {
+          // (a token that is not seen may have codes and a pair of another life, or of none: its score is -inf and its
+          // pair, which may be NaN, is taken as 0)
+#pragma unroll
+          for (int u = 0; u < NR; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int j = key0 + u * KV4_TOKENS + tok_a + half * 8;
+              if (!(j <= pos && (!BOUNDED || j >= lo || j < keep))) {
+                s[u][2 * half] = s[u][2 * half + 1] = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) vp[u][half][g] = 0u;
+              }
+            }
         }
         // the base of a head's exponents is raised only when a score has outgrown it by 2^8 (or is the first)
-        const float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
-        if (__any_sync(0xffffffffu, x0 > m[0] + 8.f || x1 > m[1] + 8.f)) {
-          float n0 = x0, n1 = x1;
+        float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]), sv = 0.f;
+#pragma unroll
+        for (int u = 1; u < NR; ++u) x0 = fmaxf(x0, fmaxf(s[u][0], s[u][2])), x1 = fmaxf(x1, fmaxf(s[u][1], s[u][3]));
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) sv = fmaxf(sv, fmaxf(kv4_s(vp[u][0][g]), kv4_s(vp[u][1][g])));
+        if (__any_sync(0xffffffffu, x0 > most[0] || x1 > most[1] || sv > s_most)) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+            sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, d));
           }
-          n0 = fmaxf(n0, m[0]), n1 = fmaxf(n1, m[1]);
-          const float f0 = m[0] == -INFINITY ? 0.f : exp2_fast(m[0] - n0);
-          const float f1 = m[1] == -INFINITY ? 0.f : exp2_fast(m[1] - n1);
-          m[0] = n0, m[1] = n1;
+          float down = s_down;
+          if (sv > s_most) {                         // (the same in all lanes: a row's pairs are its four lanes')
+            const int e = min(max((int)(__float_as_uint(sv) >> 23), 1), 247);
+            down = __uint_as_float((uint32_t)(254 - e) << 23);
+            s_most = __uint_as_float((uint32_t)(e + 6) << 23);
+          }
+          const float turn = down / s_down;
+          s_down = down;
+          x0 = fmaxf(x0, m[0]), x1 = fmaxf(x1, m[1]);
+          const float f0 = m[0] == -INFINITY ? 0.f : exp2_fast(m[0] - x0);
+          const float f1 = m[1] == -INFINITY ? 0.f : exp2_fast(m[1] - x1);
+          m[0] = x0, m[1] = x1;
+          base[0] = x0 == -INFINITY ? 0.f : x0, base[1] = x1 == -INFINITY ? 0.f : x1;
+          most[0] = x0 + 8.f, most[1] = x1 + 8.f;
           l[0] *= f0, l[1] *= f1;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             off[g][0] *= f0, off[g][1] *= f1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              ones_o[g][i] *= (i & 1) ? f1 : f0;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[g][i][c] *= (c & 1) ? f1 : f0;
-            }
+              for (int c = 0; c < 4; ++c) o[g][i][c] *= ((c & 1) ? f1 : f0) * turn;
           }
         }
-        const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
-        float p[4] = {exp2_fast(s[0] - b0), exp2_fast(s[1] - b1), exp2_fast(s[2] - b0), exp2_fast(s[3] - b1)};
-        l[0] += p[0] + p[2];
-        l[1] += p[1] + p[3];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          // (a token that is not seen may have a pair of another life, NaN too: it is taken as 0)
-          const float sa = see_a ? kv4_s(pa[NG + g]) : 0.f, sb = see_b ? kv4_s(pb[NG + g]) : 0.f;
-          const float ma = see_a ? kv4_m(pa[NG + g]) : 0.f, mb = see_b ? kv4_m(pb[NG + g]) : 0.f;
-          off[g][0] += fmaf(p[0], ma, p[2] * mb);
-          off[g][1] += fmaf(p[1], ma, p[3] * mb);
-          const uint32_t p0 = transposed8x8(pack2(p[0] * sa, p[1] * sa));
-          const uint32_t p1 = transposed8x8(pack2(p[2] * sb, p[3] * sb));
-          const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-          mma_16816(ones_o[g], one, p0, p1);
-          const uint32_t ya = __byte_perm(va[0][g], va[1][g], 0x5410), za = __byte_perm(va[0][g], va[1][g], 0x7632);
-          const uint32_t yb = __byte_perm(va[2][g], va[3][g], 0x5410), zb = __byte_perm(va[2][g], va[3][g], 0x7632);
-          const uint32_t e0[4] = {kv4_two<0>(ya), kv4_two<0>(za), kv4_two<0>(yb), kv4_two<0>(zb)};
-          mma_16816(o[g][0], e0, p0, p1);
-          const uint32_t e1[4] = {kv4_two<1>(ya), kv4_two<1>(za), kv4_two<1>(yb), kv4_two<1>(zb)};
-          mma_16816(o[g][1], e1, p0, p1);
-          const uint32_t e2[4] = {kv4_two<2>(ya), kv4_two<2>(za), kv4_two<2>(yb), kv4_two<2>(zb)};
-          mma_16816(o[g][2], e2, p0, p1);
-          const uint32_t e3[4] = {kv4_two<3>(ya), kv4_two<3>(za), kv4_two<3>(yb), kv4_two<3>(zb)};
-          mma_16816(o[g][3], e3, p0, p1);
+        for (int u = 0; u < NR; ++u) {
+          const uint8_t* b = unit + u * F::RECORD;
+          uint32_t va[4][NG];
+          load_words(b + v_at, va[0]);
+          load_words(b + v_at1, va[1]);
+          load_words(b + v_at + 8 * F::ROW, va[2]);
+          load_words(b + v_at1 + 8 * F::ROW, va[3]);
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = exp2_fast(s[u][i] - base[i & 1]);
+          l[0] += p[0] + p[2];
+          l[1] += p[1] + p[3];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const float sa = kv4_s(vp[u][0][g]), sb = kv4_s(vp[u][1][g]);
+            const float ma = fmaf(8.f, sa, kv4_m(vp[u][0][g])), mb = fmaf(8.f, sb, kv4_m(vp[u][1][g]));
+            off[g][0] = fmaf(p[2], mb, fmaf(p[0], ma, off[g][0]));
+            off[g][1] = fmaf(p[3], mb, fmaf(p[1], ma, off[g][1]));
+            const float ra = sa * s_down, rb = sb * s_down;
+            const uint32_t p0 = transposed8x8(as_u32(__floats2half2_rn(p[0] * ra, p[1] * ra)));
+            const uint32_t p1 = transposed8x8(as_u32(__floats2half2_rn(p[2] * rb, p[3] * rb)));
+            uint32_t ya[4], za[4], yb[4], zb[4];
+            kv4_codes(__byte_perm(va[0][g], va[1][g], 0x5410), magic, ya);
+            kv4_codes(__byte_perm(va[0][g], va[1][g], 0x7632), magic, za);
+            kv4_codes(__byte_perm(va[2][g], va[3][g], 0x5410), magic, yb);
+            kv4_codes(__byte_perm(va[2][g], va[3][g], 0x7632), magic, zb);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_f16(o[g][i], ya[i], za[i], yb[i], zb[i], p0, p1);
+          }
         }
+        asked &= ~(1u << stage);
+        __syncwarp();                                  // all lanes have read the stage
       }
-      asked &= ~(1u << stage);
-      __syncwarp();                                    // all lanes have read the stage
+      const int next = v + C::STAGES * C::WARPS;
+      if (next < v_end && ask(next, page_now, stage)) asked |= 1u << stage;
+      stage = stage + 1 == C::STAGES ? 0 : stage + 1;
     }
-    const int next = v + C::STAGES * C::WARPS;
-    if (next < v_end && ask(next, stage)) asked |= 1u << stage;
-    stage = stage + 1 == C::STAGES ? 0 : stage + 1;
-  }
-  if (!ok) {                                           // gave up: wait for what is still on its way, say so, go on to
-    for (int s = 0; s < C::STAGES; ++s)                // the block's barriers (the result is void)
-      if (asked >> s & 1) mbar_wait_warp(&full[warp][s], parity >> s & 1, nullptr);
-    if (lane == 0) atomicCAS(a.error, 0, GB_ERR_KV4_TIMEOUT);
-  }
-  pdl_launch_dependents();
-  if (lost) m[0] = m[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
+    if (!ok && asked) {                                // gave up: wait for what is still on its way, say so, go on to
+      for (int s = 0; s < C::STAGES; ++s)              // the block's barriers (the result is void)
+        if (asked >> s & 1) mbar_wait_warp(&full[warp][s], parity >> s & 1, nullptr);
+      if (lane == 0) atomicCAS(a.error, 0, GB_ERR_KV4_TIMEOUT);
+    }
+    if (lost) m[0] = m[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
 
-  // the sums over the rows of a head's column, and the accumulator in its own units
+    const bool again = more;
+    turn_of ^= 1;
+    if (again) part = begin();
+    else pdl_launch_dependents();
+
+    // the sums over the rows of a head's column, and the accumulator in its own units
 #pragma unroll
-  for (int d = 4; d < 32; d <<= 1) {
-    l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
-    l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+    for (int d = 4; d < 32; d <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      off[g][0] += __shfl_xor_sync(0xffffffffu, off[g][0], d);
-      off[g][1] += __shfl_xor_sync(0xffffffffu, off[g][1], d);
+      for (int g = 0; g < NG; ++g) {
+        off[g][0] += __shfl_xor_sync(0xffffffffu, off[g][0], d);
+        off[g][1] += __shfl_xor_sync(0xffffffffu, off[g][1], d);
+      }
     }
-  }
-  __syncthreads();                                     // every warp has left its ring: the results go there
-  float* red_o = reinterpret_cast<float*>(smem);       // [warps][8][D]
-  float* red_ml = red_o + C::WARPS * 8 * D;            // [warps][8][2]
+    __syncthreads();                                   // every warp has read the results of the part before
+    const float s_up = 1.f / s_down;                   // (a power of two)
 #pragma unroll
-  for (int g = 0; g < NG; ++g)
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        red_o[((size_t)warp * 8 + 2 * t + (c & 1)) * D + g * 64 + 8 * r + 2 * i + (c >> 1)] =
-            fmaf(16.f, o[g][i][c] - ones_o[g][c & 1], off[g][c & 1]);
-  if (r == 0) {
+        for (int c = 0; c < 4; ++c)
+          red_o[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + ((g * 4 + i) * 2 + (c >> 1)) * 8 + r] =
+              fmaf(s_up, o[g][i][c], off[g][c & 1]);
+    if (r == 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      red_ml[(warp * 8 + 2 * t + i) * 2] = m[i];
-      red_ml[(warp * 8 + 2 * t + i) * 2 + 1] = l[i];
+      for (int i = 0; i < 2; ++i) {
+        red_ml[(warp * 8 + 2 * t + i) * 2] = m[i];
+        red_ml[(warp * 8 + 2 * t + i) * 2 + 1] = l[i];
+      }
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
-    const int head = i / D, d = i % D;
-    float M = -INFINITY;
+    __syncthreads();
+    const Kv4Part done = part_s[turn_of ^ 1];
+    const int h0 = done.group / hgroups * G + done.group % hgroups * 8, heads = min(8, G - done.group % hgroups * 8);
+    const bool alone = done.n_pieces <= 1;             // the result is final
+    const bool live = (unsigned)a.slots[done.seq] < (unsigned)a.n_slots;
+    for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
+      const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
+      float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, red_ml[(w * 8 + head) * 2]);
-    float L = 0.f, O = 0.f;
+      for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, red_ml[(w * 8 + h) * 2]);
+      float L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      const float mw = red_ml[(w * 8 + head) * 2];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
-      L += red_ml[(w * 8 + head) * 2 + 1] * f;
-      O += red_o[((size_t)w * 8 + head) * D + d] * f;
+      for (int w = 0; w < C::WARPS; ++w) {
+        const float mw = red_ml[(w * 8 + h) * 2];
+        const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+        L += red_ml[(w * 8 + h) * 2 + 1] * f;
+        O += red_o[(w * 8 + h) * C::PITCH + place] * f;
+      }
+      const size_t row = (size_t)done.seq * a.nq + h0 + h;
+      if (alone) {
+        if (a.sinks && live && a.sinks[h0 + h] != -INFINITY) O *= add_sink(a.sinks[h0 + h], M, L);
+        reinterpret_cast<bf16*>(a.out)[row * D + d] = __float2bfloat16(L != 0.f ? O / L : 0.f);
+        if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+      } else if (done.piece < a.n_splits) {            // (more than the caller's bound of the lengths allows: merged as NaN)
+        a.part_o[(row * a.n_splits + done.piece) * D + d] = O;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.n_splits + done.piece) * 2) = make_float2(M, L);
+      }
     }
-    const size_t row = (size_t)seq * a.nq + h0 + head;
-    if (a.n_splits == 1) {
-      if (a.sinks && live && a.sinks[h0 + head] != -INFINITY) O *= add_sink(a.sinks[h0 + head], M, L);
-      reinterpret_cast<bf16*>(a.out)[row * D + d] = __float2bfloat16(L != 0.f ? O / L : 0.f);
-      if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
-    } else {
-      a.part_o[(row * a.n_splits + split) * D + d] = O;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.n_splits + split) * 2) = make_float2(M, L);
-    }
+    if (a.n_splits > 1 && done.piece == 0 && threadIdx.x == 0) a.pieces[done.seq * groups + done.group] = done.n_pieces;
+    if (!again) break;
   }
 }
 
-// out[row] from the partial results of the splits, in their order; one block a (row, head).
+// out[row] from the partial results of its splits, in their order; one block a (row, head).  Rows of one split are
+// finished already.
 template <typename T>
-__global__ void kv4_merge_kernel(const Kv4AttnArgs a, int D) {
-  pdl_wait();
+__global__ void kv4_merge_kernel(const Kv4AttnArgs a, int D, int per_group) {
   const size_t row = blockIdx.x, p0 = row * a.n_splits;
-  const int seq = a.row_seq ? a.row_seq[row / a.nq] : (int)(row / a.nq);
-  const bool live = (unsigned)seq < (unsigned)a.n_seqs && (unsigned)a.slots[seq] < (unsigned)a.n_slots;
+  const int d = threadIdx.x, G = a.nq / a.nkv, hgroups = (G + per_group - 1) / per_group, h = row % a.nq;
+  const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
+  pdl_wait();                                        // (every block: the next kernel waits for this one only)
+  const int n = a.pieces[row / a.nq * a.nkv * hgroups + h / G * hgroups + h % G / per_group];
+  if (n <= 1) return;
+  if (n > a.n_splits) {                               // keys beyond the caller's bound: some were left out
+    reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(__int_as_float(0x7fffffff));
+    if (a.lse && d == 0) a.lse[row] = __int_as_float(0x7fffffff);
+    return;
+  }
+  // (loads are requested eight splits at a time and used in split order)
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
-  float M = -INFINITY;
-  for (int s = 0; s < a.n_splits; ++s) M = fmaxf(M, ml[s].x);
-  const float sink = a.sinks && live ? a.sinks[row % a.nq] * 1.4426950408889634f : -INFINITY;
-  M = fmaxf(M, sink);
-  const int d = threadIdx.x;
-  float L = sink == -INFINITY ? 0.f : exp2f(sink - M), O = 0.f;
-  for (int s = 0; s < a.n_splits; ++s) {
-    const float2 v = ml[s];
-    if (v.x == -INFINITY) continue;
-    const float f = exp2f(v.x - M);
-    L += v.y * f;
-    O += a.part_o[(p0 + s) * D + d] * f;
+  float M = sk, L = 0.f, O = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = ml[min(s0 + u, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) M = fmaxf(M, v[u].x);
+  }
+  if (sk != -INFINITY) L = exp2f(sk - M);
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float2 v[8];
+    float o[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = min(s0 + u, n - 1);
+      v[u] = ml[s];
+      o[u] = a.part_o[(p0 + s) * D + d];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + u < n && v[u].x != -INFINITY) {
+        const float f = exp2f(v[u].x - M);
+        L += v[u].y * f;
+        O += o[u] * f;
+      }
+    }
   }
   reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(L != 0.f ? O / L : 0.f);
   if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
@@ -433,16 +715,14 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
   const int row = blockIdx.x / a.n_splits, split = blockIdx.x % a.n_splits;
   const int kvh = blockIdx.y / hgroups, hg = blockIdx.y % hgroups;
   const int h0 = kvh * G + hg * HC, heads = min(HC, G - hg * HC);
-  const int seq = a.row_seq ? a.row_seq[row] : row;
-  const bool known = (unsigned)seq < (unsigned)a.n_seqs;
-  const int slot = known ? a.slots[seq] : -1;
-  const bool live = (unsigned)slot < (unsigned)a.n_slots;
-  const int behind = a.row_seq && known ? a.cu_q[seq + 1] - 1 - row : 0;    // rows of the sequence behind this one
-  const int pos = live ? a.kv_len[seq] - 1 - behind : -1;
+  int pos;
+  const bool live = find_row(a, row, pos);
+  const int slot = live ? a.slots[a.row_seq ? a.row_seq[row] : row] : -1;
   const Stretches list(pos, 32, a.window, a.keep_first, a.chunk);
   const int keep = a.window > 0 ? a.keep_first : 0;
-  const int per = (list.n + a.n_splits - 1) / a.n_splits;
-  const int v_end = min(list.n, (split + 1) * per);
+  const int v_end = a.n_splits == 1 ? list.n : min(list.n, (split + 1) * a.per);
+  if (split > 0 && split * a.per >= list.n) return;
+  const bool alone = a.n_splits == 1 || list.n <= a.per;
   const int* table = a.block_table + (size_t)(live ? slot : 0) * a.max_pages;
   for (int i = threadIdx.x; i < HC * D; i += blockDim.x)
     q_s[i / D][i % D] = i / D < heads ? reinterpret_cast<const float*>(a.q)[((size_t)row * a.nq + h0) * D + i] : 0.f;
@@ -461,7 +741,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
     for (int e = 0; e < 8; ++e) o[h][e] = 0.f;
   }
   const int word = lane % LANES, half = lane / LANES, group = word / 8;   // this lane's elements of a value
-  for (int v = split * per + warp; v < v_end; v += KV4_F32_WARPS) {
+  for (int v = split * a.per + warp; v < v_end; v += KV4_F32_WARPS) {
     const int key0 = list.at(v) * 32, key = key0 + lane;
     const int page = kv4_page(table, key0 / KV4_PAGE, a.max_pages, a.n_pages);
     if (page < 0) {                                        // a page that there is not: the result is NaN
@@ -570,7 +850,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       O += red_o[w][head][d] * f;
     }
     const size_t at = (size_t)row * a.nq + h0 + head;
-    if (a.n_splits == 1) {
+    if (alone) {
       if (a.sinks && live && a.sinks[h0 + head] != -INFINITY) O *= add_sink(a.sinks[h0 + head], M, L);
       reinterpret_cast<float*>(a.out)[at * D + d] = L != 0.f ? O / L : 0.f;
       if (a.lse && d == 0) a.lse[at] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
@@ -579,6 +859,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.n_splits + split) * 2) = make_float2(M, L);
     }
   }
+  if (a.n_splits > 1 && split == 0 && threadIdx.x == 0) a.pieces[(size_t)row * gridDim.y + blockIdx.y] = max(1, (list.n + a.per - 1) / a.per);
 }
 
 // ---------------------------------------------------------------- the weights that tokens gather
@@ -619,6 +900,7 @@ __global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4We
   const int lowest = first_key(max(pos0, 0), a.window, a.chunk);  // no row sees a key below it but for the kept ones
   const int keep = a.window > 0 ? a.keep_first : 0;
   const int records = (len + KV4_TOKENS - 1) / KV4_TOKENS;
+  const uint32_t magic = kv4_magic(a.n_seqs);
   for (int rec = blockIdx.x * WEIGH_WARPS + warp; rec < records; rec += gridDim.x * WEIGH_WARPS) {
     const int key0 = rec * KV4_TOKENS;
     if (key0 + KV4_TOKENS <= lowest && key0 >= keep) continue;
@@ -639,16 +921,16 @@ __global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4We
       if (!__any_sync(0xffffffffu, see_a || see_b)) continue;
       for (int hc = 0; hc < G; hc += 8) {
         const int h0 = kvh * G + hc, heads = min(8, G - hc);
-        uint32_t q[D / 32][4];
-        float qsum[NG][2], s[4];
-        kv4_query<D>(r < heads ? a.q + ((size_t)row * a.nq + h0 + r) * D : nullptr, q, qsum);
-        kv4_scores<D>(ka, kb, pa, pb, q, qsum, s);
+        Kv4Query<D> q;
+        float s[4];
+        q.load(r < heads ? a.q + ((size_t)row * a.nq + h0 + r) * D : nullptr);
+        kv4_scores<D>(ka, kb, pa, pb, q, magic, s);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float lse = 2 * t + i < heads ? a.lse[(size_t)row * a.nq + h0 + 2 * t + i] * 1.4426950408889634f : -INFINITY;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float x = s[2 * half + i];
+            const float x = s[2 * half + i] * q.back[i];
             const float y = a.cap.cap_log2 != 0.f ? capped_log2(x * a.cap.cap_inv, a.cap) : x * a.scale_log2;
             if (lse != -INFINITY && (half ? see_b : see_a)) (half ? wb : wa) += exp2f(y - lse);
           }
@@ -667,41 +949,51 @@ __global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4We
 static int checked(const Kv4AttnArgs* a, int D) {
   if (D != 64 && D != 128) return GB_ERR_UNSUPPORTED;
   if (!a->q || !a->pages || !a->out || !a->block_table || !a->slots || !a->kv_len || a->n_rows < 0 || a->n_seqs < 0 ||
-      a->nq <= 0 || a->nkv <= 0 || a->nq % a->nkv || a->max_pages <= 0 || a->n_pages <= 0 || a->n_slots < 0 ||
-      a->n_splits <= 0 || a->chunk < 0 || a->window < 0 || a->keep_first < 0)
+      a->nq <= 0 || a->nkv <= 0 || a->nq % a->nkv || a->max_pages <= 0 || a->max_pages > 0x1000000 || a->n_pages <= 0 || a->n_slots < 0 ||
+      a->n_splits <= 0 || a->per <= 0 || a->chunk < 0 || a->window < 0 || a->keep_first < 0)
     return GB_ERR_BAD_ARG;
-  if (a->n_splits > 1 && (!a->part_o || !a->part_ml)) return GB_ERR_BAD_ARG;
+  if (a->n_splits > 1 && (!a->part_o || !a->part_ml || !a->pieces)) return GB_ERR_BAD_ARG;
   if (((uintptr_t)a->q | (uintptr_t)a->pages) & 15) return GB_ERR_BAD_ARG;
   return 0;
 }
 
-// The shared-memory size is a property of a kernel on one device; it is set once on each.
-template <int D>
-static int decode(const Kv4AttnArgs& a, cudaStream_t s) {
-  static bool configured[64] = {};
+template <int D, bool BOUNDED>
+static int decode_launch(const Kv4AttnArgs& a, unsigned grid, cudaStream_t s) {
+  static bool configured[64] = {};     // (the shared-memory size is a property of a kernel on one device)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kv4_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv4Decode<D>::SMEM);
+    e = cudaFuncSetAttribute(kv4_decode_kernel<D, BOUNDED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Kv4Decode<D>::SMEM);
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) configured[dev] = true;
   }
-  const int hgroups = (a.nq / a.nkv + 7) / 8;
-  if ((long long)a.nkv * hgroups > 65535 || a.n_seqs > 65535) return GB_ERR_UNSUPPORTED;
-  int rc = gb_launch(kv4_decode_kernel<D>, dim3(a.n_splits, a.nkv * hgroups, a.n_seqs), dim3(Kv4Decode<D>::WARPS * 32),
-                     Kv4Decode<D>::SMEM, s, a);
-  if (rc || a.n_splits == 1) return rc;
-  return gb_launch(kv4_merge_kernel<bf16>, dim3((unsigned)(a.n_rows * a.nq)), dim3(D), 0, s, a, D);
+  return gb_launch(kv4_decode_kernel<D, BOUNDED>, dim3(grid), dim3(Kv4Decode<D>::WARPS * 32), Kv4Decode<D>::SMEM, s, a);
 }
 
-GB_EXPORT int gb_attn_kv4_decode(const Kv4AttnArgs* a, int D, cudaStream_t s) {
+template <int D>
+static int decode(const Kv4AttnArgs& a, int blocks, cudaStream_t s) {
+  const int hgroups = (a.nq / a.nkv + 7) / 8;
+  const long long pairs = (long long)a.nkv * hgroups * a.n_seqs;
+  if (pairs * a.n_splits > 0x7fffffffll) return GB_ERR_UNSUPPORTED;
+  // (all stretches are counted in 32 bits, and a block's run may reach beyond them)
+  if (a.shared && (a.n_splits < 2 || a.n_seqs > KV4_SHARED_SEQS || blocks <= 0 ||
+                   pairs * (4ll * a.max_pages + 4) + 2ll * blocks * a.per > 0x7fffffffll))
+    return GB_ERR_BAD_ARG;
+  const unsigned grid = (unsigned)(a.shared ? blocks : pairs * a.n_splits);
+  const int rc = a.window > 0 || a.chunk > 0 ? decode_launch<D, true>(a, grid, s) : decode_launch<D, false>(a, grid, s);
+  if (rc || a.n_splits == 1) return rc;
+  return gb_launch(kv4_merge_kernel<bf16>, dim3((unsigned)(a.n_rows * a.nq)), dim3(D), 0, s, a, D, 8);
+}
+
+// `blocks`: how many share the keys out (a->shared).
+GB_EXPORT int gb_attn_kv4_decode(const Kv4AttnArgs* a, int D, int blocks, cudaStream_t s) {
   const int rc = checked(a, D);
   if (rc) return rc;
   if (!a->error || a->n_rows != a->n_seqs || a->row_seq) return GB_ERR_BAD_ARG;
   if ((long long)a->n_rows * a->nq > 0x7fffffffll) return GB_ERR_UNSUPPORTED;
   if (a->n_rows == 0) return 0;
-  return D == 64 ? decode<64>(*a, s) : decode<128>(*a, s);
+  return D == 64 ? decode<64>(*a, blocks, s) : decode<128>(*a, blocks, s);
 }
 
 GB_EXPORT int gb_attn_kv4_f32(const Kv4AttnArgs* a, int D, cudaStream_t s) {
@@ -717,7 +1009,7 @@ GB_EXPORT int gb_attn_kv4_f32(const Kv4AttnArgs* a, int D, cudaStream_t s) {
   rc = D == 64 ? gb_launch(kv4_f32_kernel<64>, grid, dim3(KV4_F32_WARPS * 32), 0, s, *a)
                : gb_launch(kv4_f32_kernel<128>, grid, dim3(KV4_F32_WARPS * 32), 0, s, *a);
   if (rc || a->n_splits == 1) return rc;
-  return gb_launch(kv4_merge_kernel<float>, dim3((unsigned)(a->n_rows * a->nq)), dim3(D), 0, s, *a, D);
+  return gb_launch(kv4_merge_kernel<float>, dim3((unsigned)(a->n_rows * a->nq)), dim3(D), 0, s, *a, D, KV4_F32_HEADS);
 }
 
 // `blocks`: blocks along the keys of every (kv head, sequence).

@@ -1908,22 +1908,39 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
 
 class _Kv4AttnArgs(ctypes.Structure):
     _fields_ = [("q", _P), ("pages", _P), ("block_table", _P), ("slots", _P), ("kv_len", _P), ("row_seq", _P),
-                ("cu_q", _P), ("out", _P), ("lse", _P), ("part_o", _P), ("part_ml", _P), ("error", _P),
-                ("sinks", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
-                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("n_splits", _I), ("keep_first", _I), ("chunk", _I),
-                ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
+                ("cu_q", _P), ("out", _P), ("lse", _P), ("part_o", _P), ("part_ml", _P), ("pieces", _P),
+                ("error", _P), ("sinks", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
+                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("n_splits", _I), ("per", _I), ("shared", _I),
+                ("keep_first", _I),
+                ("chunk", _I), ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
 
 
-def kv4_splits(pairs: int, max_kv_len: int, device) -> int:
-    """How many ways the keys of a sequence are split, for ``pairs`` (sequence, group of query heads) pairs."""
-    if DECODE_SPLITS_OVERRIDE:
-        return DECODE_SPLITS_OVERRIDE
-    places = 2 * _sm_count(device)
-    tiles = max(1, (max_kv_len + 63) // 64)
-    most = max(1, min(64, (tiles + 3) // 4))
-    cost = {s: ((pairs * s + places - 1) // places) * (-(-tiles // (4 * s)) + 2.0) for s in range(1, most + 1)}
-    best = min(cost.values())
-    return min(s for s, c in cost.items() if c <= 1.03 * best)
+KV4_LEAST = 8              # stretches of 32 keys that a block takes at least (two for each of its warps)
+KV4_WHOLE = 16             # up to so many a block takes all of a pair
+KV4_SPLIT_OVERRIDE: Optional[int] = None      # stretches that a block takes at least, for experiments
+KV4_SHARE_OVERRIDE: Optional[bool] = None     # whether they are shared out, for tests
+
+
+def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int) -> Tuple[int, int, int]:
+    """(splits, stretches of 32 keys, blocks) of the bfloat16 kernel for ``pairs`` (sequence, group of query heads)
+    pairs of up to ``keys`` keys.  One split: a block a pair.  More and no blocks: a block a split of so many stretches.
+    With blocks: they share the stretches out, at least so many each, and a pair has at most so many of them."""
+    tiles = max(1, (keys + 31) // 32)
+    least = KV4_SPLIT_OVERRIDE or (tiles if tiles <= KV4_WHOLE else max(KV4_LEAST, -(-tiles // 62)))
+    if tiles <= least:
+        return 1, tiles, 0
+    splits, blocks = -(-tiles // least), 4 * sms
+    share = splits * pairs > blocks if KV4_SHARE_OVERRIDE is None else KV4_SHARE_OVERRIDE
+    if share and n_seqs <= 256 and pairs * (4 * max_pages + 4) + 2 * blocks * least <= 0x7fffffff:
+        return min(blocks, splits + 1), least, blocks
+    return splits, least, 0
+
+
+def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int]:
+    """(splits, stretches of 32 keys in a split) of the 32-bit kernel."""
+    tiles = max(1, (keys + 31) // 32)
+    per = KV4_SPLIT_OVERRIDE or max(8, -(-tiles * pairs // (8 * sms)), -(-tiles // 64))
+    return -(-tiles // per), per
 
 
 def _kv4_query(q, pages, block_table, step, page: int, softcap, window, keep_first, chunk):
@@ -2006,11 +2023,16 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         a.row_seq = step.token_seq.data_ptr()
     per = 4 if f32 else 8
     groups = nkv * ((nq // nkv + per - 1) // per)
-    ns = kv4_splits((T if f32 else n_seqs) * groups, _keys_visited(step.max_kv_len, window, page, keep_first, int(chunk or 0)),
-                    q.device)
+    keys = _keys_visited(step.max_kv_len, window, page, keep_first, int(chunk or 0))
+    if f32:
+        ns, a.per = kv4_split_plan_f32(T * groups, keys, _sm_count(q.device))
+    else:
+        ns, a.per, blocks = kv4_split_plan(n_seqs, n_seqs * groups, keys, block_table.shape[1], _sm_count(q.device))
+        a.shared = int(blocks > 0)
     if ns > 1:       # (memory of this call's own: two captured graphs, or two streams, share none of it)
-        part = torch.empty(T * nq * ns * (D + 2), dtype=torch.float32, device=q.device)
-        a.part_o, a.part_ml = part.data_ptr(), part[T * nq * ns * D:].data_ptr()
+        part = torch.empty(T * nq * ns * (D + 2) + T * groups, dtype=torch.float32, device=q.device)
+        a.part_o, a.part_ml = part.data_ptr(), part.data_ptr() + 4 * T * nq * ns * D
+        a.pieces = part.data_ptr() + 4 * T * nq * ns * (D + 2)
     a.q, a.pages, a.block_table, a.slots = q.data_ptr(), pages.data_ptr(), block_table.data_ptr(), step.slots.data_ptr()
     a.kv_len, a.cu_q, a.out, a.lse = step.kv_len.data_ptr(), step.cu_q.data_ptr(), out.data_ptr(), _ptr(lse)
     a.error = _tc_error_flag(q.device).data_ptr()
@@ -2018,10 +2040,13 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     a.max_pages, a.n_pages, a.window, a.n_splits = block_table.shape[1], n_pages, int(window or 0), ns
     a.keep_first, a.chunk, a.scale_log2 = keep_first, int(chunk or 0), float(scale) * _LOG2E
     _set_cap_and_sinks(a, scale, softcap, sinks, nq)
-    name = "f32" if f32 else "decode"
     with _on(q):
-        _check(_fn("attn_kv4", "gb_attn_kv4_" + name, "pip")(ctypes.addressof(a), D, _stream()), "attn_kv4_" + name,
-               2 if ns > 1 else 1)
+        if f32:
+            _check(_fn("attn_kv4", "gb_attn_kv4_f32", "pip")(ctypes.addressof(a), D, _stream()), "attn_kv4_f32",
+                   2 if ns > 1 else 1)
+        else:
+            _check(_fn("attn_kv4", "gb_attn_kv4_decode", "piip")(ctypes.addressof(a), D, blocks, _stream()),
+                   "attn_kv4_decode", 2 if ns > 1 else 1)
     return (out, lse) if want_lse else out
 
 

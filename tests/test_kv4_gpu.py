@@ -219,10 +219,10 @@ def test_single_tokens(lens, nq, nkv, D, dtype, seen):
     attend(c, [1] * len(lens), nq, dtype, sinks=len(lens) % 2 == 1, pad=len(lens) % 3, **seen)
 
 
-@pytest.mark.parametrize("splits", [1, 2, 5, 64])
+@pytest.mark.parametrize("stretches", [1, 3, 4, 8, 100])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_splits_of_the_keys(splits, dtype, monkeypatch):
-    monkeypatch.setattr(ops, "DECODE_SPLITS_OVERRIDE", splits)
+def test_splits_of_the_keys(stretches, dtype, monkeypatch):
+    monkeypatch.setattr(ops, "KV4_SPLIT_OVERRIDE", stretches)
     c = Cache([1000, 1, 130], 2, 128, dtype)
     attend(c, [1, 1, 1], 8, dtype, sinks=True, pad=1)
     attend(c, [1, 1, 1], 8, dtype, window=200, keep_first=3)
@@ -243,6 +243,30 @@ def test_prompts_in_large_blocks(n):
     """Enough rows and heads that a block takes 256 query rows."""
     c = Cache([n, n // 3], 8, 128, seed=n)
     attend(c, [n, n // 3], 32, torch.bfloat16)
+
+
+@pytest.mark.parametrize("lens", [[3000, 1, 200, 64, 2500], [33] * 40 + [2000], [700], [2100, 2100, 2100]], ids=lambda x: str(len(x)))
+@pytest.mark.parametrize("least,share", [(None, None), (2, True), (3, True), (9, True), (1, True), (5, False)])
+def test_keys_shared_out_among_the_blocks(lens, least, share, monkeypatch):
+    """Runs of stretches that end inside a pair, hold several pairs, or one pair's middle; padding rows between."""
+    monkeypatch.setattr(ops, "KV4_SPLIT_OVERRIDE", least)
+    monkeypatch.setattr(ops, "KV4_SHARE_OVERRIDE", share)
+    c = Cache(lens, 2, 64, seed=len(lens))
+    attend(c, [1] * len(lens), 12, torch.bfloat16, sinks=True, pad=2)
+    attend(c, [1] * len(lens), 4, torch.bfloat16, window=300, keep_first=40)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bound", [1, 700, 1500])
+def test_a_bound_of_the_lengths_that_is_too_low(dtype, bound):
+    """Rows with more keys than the caller's bound are right or NaN, and the others right."""
+    c = Cache([3000, 90], 2, 64, dtype, seed=3)
+    step, q = c.step([1, 1]), queries(2, 8, 64, dtype, 0).to(DEV)
+    want = ops.attention_kv4(q, c.pages, c.table, step=step, page=64, scale=0.1)
+    step.max_kv_len = bound
+    got = ops.attention_kv4(q, c.pages, c.table, step=step, page=64, scale=0.1)
+    assert bool(got[0].isnan().all()) or float((got[0] - want[0]).abs().max()) < 0.01
+    assert float((got[1] - want[1]).abs().max()) < 0.01
 
 
 def test_a_capped_score_far_beyond_the_cap():
