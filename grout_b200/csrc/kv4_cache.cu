@@ -386,24 +386,32 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
   }
 }
 
-GB_EXPORT int gb_kv4_choose(const Kv4ChooseArgs* a, cudaStream_t s) {
+static int choose(const Kv4ChooseArgs* a, cudaStream_t s) {
   if (a->n_seqs < 0 || a->nkv <= 0 || a->max_pages <= 0 || a->max_pages > 0x7fffffff / KV4_PAGE || a->n_pages <= 0 ||
-      a->first < 0 || a->recent < 0 || a->keep <= 0 || a->first + a->recent > a->keep)
+      a->first < 0 || a->recent < 0 || a->keep <= 0 || a->first > a->keep || a->recent > a->keep - a->first)
     return GB_ERR_BAD_ARG;
   if (a->n_seqs > GB_MAX_GRID_YZ) return GB_ERR_UNSUPPORTED;
-  if (a->n_seqs == 0) return 0;
   return gb_launch(kv4_choose_kernel, dim3(a->nkv, a->n_seqs), dim3(CHOOSE_THREADS), 0, s, *a);
 }
 
-GB_EXPORT int gb_kv4_move(const Kv4MoveArgs* a, int D, cudaStream_t s) {
-  if (a->n_seqs < 0 || a->nkv <= 0 || a->keep <= 0 || !a->from || !a->to || !a->kept ||
+static int move(const Kv4MoveArgs* a, int D, cudaStream_t s) {
+  if (a->n_seqs < 0 || a->nkv <= 0 || a->keep <= 0 || a->keep > 0x7fffff00 || !a->from || !a->to || !a->kept ||
       (((uintptr_t)a->from | (uintptr_t)a->to) & 15))
     return GB_ERR_BAD_ARG;
   if (a->nkv > GB_MAX_GRID_YZ || a->n_seqs > GB_MAX_GRID_YZ) return GB_ERR_UNSUPPORTED;
-  if (a->n_seqs == 0) return 0;
   const int n_rec = (a->keep + KV4_TOKENS - 1) / KV4_TOKENS;
   const dim3 grid((n_rec + 3) / 4, a->nkv, a->n_seqs);
   if (D == 64) return gb_launch(kv4_move_kernel<64>, grid, dim3(128), 0, s, *a);
   if (D == 128) return gb_launch(kv4_move_kernel<128>, grid, dim3(128), 0, s, *a);
   return GB_ERR_UNSUPPORTED;
+}
+
+// The choice, then the kept tokens moved: straight to their pages, or (back not null) out of the pages and back.
+GB_EXPORT int gb_kv4_evict(const Kv4ChooseArgs* c, const Kv4MoveArgs* out, const Kv4MoveArgs* back, int D, cudaStream_t s) {
+  if (c->n_seqs == 0) return 0;
+  if (D != 64 && D != 128) return GB_ERR_UNSUPPORTED;
+  int rc = choose(c, s);
+  if (!rc) rc = move(out, D, s);
+  if (!rc && back) rc = move(back, D, s);
+  return rc;
 }

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Tuple
 
@@ -1798,8 +1799,11 @@ def attention(q, k_pages, v_pages, block_table, *, step, page: int, scale: float
 
 
 # ---------------------------------------------------------------- a cache in 4 bits
+# (A decode step's calls take a few microseconds on the device, so what stands in front of them counts: a tensor's type,
+# place and order are looked at once, arguments are packed in one go, and the stream is asked for by device number.)
 _TC_ERROR_NAMES[141] = "a warp of the 4-bit decode attention waited 2 s for keys that never arrived"
 KV4_PAGE = 64              # tokens of a page
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
 
 def kv4_record(D: int) -> int:
@@ -1815,56 +1819,64 @@ def kv4_pages(n_pages: int, nkv: int, D: int, device) -> torch.Tensor:
     return torch.zeros((n_pages, nkv, 4, kv4_record(D)), dtype=torch.uint8, device=device)
 
 
-def _kv4_pages_of(pages, device=None):
-    """(pages, kv heads, D) of a 4-bit cache's pages."""
-    _need(pages, "4-bit pages", torch.uint8, 4)
-    n, nkv, four, record = pages.shape
-    if four != 4 or record not in (18 * 64, 18 * 128) or n < 1 or nkv < 1 or pages.data_ptr() % 16:
-        raise KernelError(f"4-bit pages are {tuple(pages.shape)}, expected [pages, kv heads, 4, {18 * 64} or {18 * 128}]")
-    return n, nkv, record // 18
+def _take(t: torch.Tensor, name: str, dtype, ndim: int, dev: int) -> int:
+    """A contiguous tensor's address, when it has this type and is on this device."""
+    if t is not None and t.dtype is dtype and t.dim() == ndim and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    _need(t, name, dtype, ndim)
+    raise KernelError(f"{name} is on {t.device}, other tensors of the call on cuda:{dev}")
 
 
-def _same_device(t: torch.Tensor, *others) -> None:
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise KernelError(f"tensors on {t.device} and on {o.device}")
+def _take16(t: torch.Tensor, name: str, dtype, ndim: int, dev: int) -> int:
+    p = _take(t, name, dtype, ndim, dev)
+    if p % 16:
+        raise KernelError(f"{name} must start on 16 bytes")
+    return p
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device made the current one, so that the launch goes to its current stream."""
-    return torch.cuda.device(t.device)
-
-
-class _Kv4RowsArgs(ctypes.Structure):
-    _fields_ = [("kv", _P), ("out", _P), ("token_seq", _P), ("token_pos", _P), ("slots", _P), ("block_table", _P),
-                ("pages", _P), ("weights", _P), ("T", _I), ("n_seqs", _I), ("n_slots", _I), ("nkv", _I),
-                ("max_pages", _I), ("n_pages", _I)]
-
-
-def _kv4_rows_args(pages, weights, token_seq, token_pos, slots, block_table, page: int):
-    n_pages, nkv, D = _kv4_pages_of(pages)
+def _kv4_pages_of(pages, page: int):
+    """(device number, address, pages, kv heads, D) of a 4-bit cache's pages."""
     if page != KV4_PAGE:
         raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
-    for t, nm in ((token_seq, "token_seq"), (token_pos, "token_pos"), (slots, "slots")):
-        _need(t, nm, torch.int32, 1)
-    _need(block_table, "block table", torch.int32, 2)
-    if token_pos.shape[0] != token_seq.shape[0]:
-        raise KernelError(f"{token_seq.shape[0]} tokens have {token_pos.shape[0]} positions")
-    if weights is not None:
-        _check_kv4_weights(weights, pages)
-    _same_device(pages, token_seq, token_pos, slots, block_table, weights)
-    a = _Kv4RowsArgs()
-    a.token_seq, a.token_pos, a.slots = token_seq.data_ptr(), token_pos.data_ptr(), slots.data_ptr()
-    a.block_table, a.pages, a.weights = block_table.data_ptr(), pages.data_ptr(), _ptr(weights)
-    a.T, a.n_seqs, a.n_slots, a.nkv = token_seq.shape[0], slots.shape[0], block_table.shape[0], nkv
-    a.max_pages, a.n_pages = block_table.shape[1], n_pages
-    return a, nkv, D
+    dev = pages.get_device()
+    p = _take16(pages, "4-bit pages", torch.uint8, 4, dev if dev >= 0 else 0)
+    n, nkv, four, record = pages.shape
+    if four != 4 or record not in (18 * 64, 18 * 128) or n < 1 or nkv < 1:
+        raise KernelError(f"4-bit pages are {tuple(pages.shape)}, expected [pages, kv heads, 4, {18 * 64} or {18 * 128}]")
+    return dev, p, n, nkv, record // 18
 
 
-def _check_kv4_weights(weights, pages) -> None:
-    _need(weights, "token weights", torch.float32, 3)
-    if tuple(weights.shape) != (pages.shape[0], pages.shape[1], KV4_PAGE):
-        raise KernelError(f"token weights are {tuple(weights.shape)}, expected {(pages.shape[0], pages.shape[1], KV4_PAGE)}")
+def _take_weights(weights, n_pages: int, nkv: int, dev: int) -> int:
+    p = _take(weights, "token weights", _F32, 3, dev)
+    if weights.shape != (n_pages, nkv, KV4_PAGE):
+        raise KernelError(f"token weights are {tuple(weights.shape)}, expected {(n_pages, nkv, KV4_PAGE)}")
+    return p
+
+
+def _launch(dev: int, what: str, kernels: int, fn, *args) -> None:
+    """Calls a kernel's entry point on the current stream of device ``dev``."""
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    _check(rc, what, kernels)
+
+
+_KV4_ROWS = struct.Struct("@8P6i")
+
+
+def _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page: int):
+    """What reading and writing rows share: (device, kv heads, D, rows, the arguments behind the rows' two addresses)."""
+    dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
+    seq, pos = _take(token_seq, "token_seq", _I32, 1, dev), _take(token_pos, "token_pos", _I32, 1, dev)
+    sl, table = _take(slots, "slots", _I32, 1, dev), _take(block_table, "block table", _I32, 2, dev)
+    T = token_seq.shape[0]
+    if token_pos.shape[0] != T:
+        raise KernelError(f"{T} tokens have {token_pos.shape[0]} positions")
+    w = 0 if weights is None else _take_weights(weights, n_pages, nkv, dev)
+    n_slots, max_pages = block_table.shape
+    return dev, nkv, D, T, (seq, pos, sl, table, p, w, T, slots.shape[0], n_slots, nkv, max_pages, n_pages)
 
 
 @_profiled("kv4_write", lambda out, kv, *a, **k: (_nbytes(kv) + kv.numel() * 9 // 16, 0))
@@ -1876,18 +1888,12 @@ def kv4_write(kv: torch.Tensor, nkv: int, D: int, *, token_seq, token_pos, slots
     rounded up; they are read as s c + m, at most s / 2 off.  64 elements of which one is not finite, or whose range
     bfloat16 does not hold, are read as NaN.  Rows of slot -1 and places outside the block table store nothing; two
     rows of one call must not have the same place.  ``weights`` (``kv4_weigh``): the new tokens' are set to 0."""
-    _need(kv, "kv rows", ndim=3)
-    a, n, d = _kv4_rows_args(pages, weights, token_seq, token_pos, slots, block_table, page)
-    if (n, d) != (nkv, D) or tuple(kv.shape) != (a.T, 2 * nkv, D):
-        raise KernelError(f"kv rows are {tuple(kv.shape)} for pages of {n} kv heads of {d}, expected [{a.T}, {2 * nkv}, {D}]")
-    if kv.data_ptr() % 16:
-        raise KernelError("kv rows must start on 16 bytes")
-    _same_device(pages, kv)
-    a.kv = kv.data_ptr()
+    dev, n, d, T, rest = _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page)
+    if kv.dim() != 3 or (n, d) != (nkv, D) or kv.shape != (T, 2 * nkv, D):
+        raise KernelError(f"kv rows are {tuple(kv.shape)} for pages of {n} kv heads of {d}, expected [{T}, {2 * nkv}, {D}]")
     f32 = _suffix(kv.dtype) == "f32"
-    with _on(kv):
-        _check(_fn("kv4_cache", "gb_kv4_write", "piip")(ctypes.addressof(a), D, int(f32), _stream()), "kv4_write",
-               1 if a.T else 0)
+    src = _take16(kv, "kv rows", kv.dtype, 3, dev)
+    _launch(dev, "kv4_write", 1 if T else 0, _fn("kv4_cache", "gb_kv4_write", "piip"), _KV4_ROWS.pack(src, 0, *rest), D, f32)
 
 
 @_profiled("kv4_read", lambda out, pages, **k: (_nbytes(out) + out.numel() * 9 // 16, 0))
@@ -1896,23 +1902,12 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
     """The keys and values [T, 2 nkv, D] that a 4-bit cache holds at the given places, as ``kv4_write`` takes them
     (``dtype`` bfloat16 or float32: s c + m in 32 bits, rounded once).  Zeros for rows of slot -1 and places outside
     the block table."""
-    a, nkv, D = _kv4_rows_args(pages, None, token_seq, token_pos, slots, block_table, page)
+    dev, nkv, D, T, rest = _kv4_rows(pages, None, token_seq, token_pos, slots, block_table, page)
     f32 = _suffix(dtype) == "f32"
-    out = torch.empty((a.T, 2 * nkv, D), dtype=dtype, device=pages.device)
-    a.out = out.data_ptr()
-    with _on(pages):
-        _check(_fn("kv4_cache", "gb_kv4_read", "piip")(ctypes.addressof(a), D, int(f32), _stream()), "kv4_read",
-               1 if a.T else 0)
+    out = torch.empty((T, 2 * nkv, D), dtype=dtype, device=pages.device)
+    _launch(dev, "kv4_read", 1 if T else 0, _fn("kv4_cache", "gb_kv4_read", "piip"),
+            _KV4_ROWS.pack(0, out.data_ptr(), *rest), D, f32)
     return out
-
-
-class _Kv4AttnArgs(ctypes.Structure):
-    _fields_ = [("q", _P), ("pages", _P), ("block_table", _P), ("slots", _P), ("kv_len", _P), ("row_seq", _P),
-                ("cu_q", _P), ("out", _P), ("lse", _P), ("part_o", _P), ("part_ml", _P), ("pieces", _P),
-                ("error", _P), ("sinks", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
-                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("n_splits", _I), ("per", _I), ("shared", _I),
-                ("keep_first", _I),
-                ("chunk", _I), ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
 
 
 KV4_LEAST = 8              # stretches of 32 keys that a block takes at least (two for each of its warps)
@@ -1943,35 +1938,39 @@ def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int]:
     return -(-tiles // per), per
 
 
-def _kv4_query(q, pages, block_table, step, page: int, softcap, window, keep_first, chunk):
-    """The checks that everything shares that takes queries over a 4-bit cache; its sizes."""
-    _need(q, "q", ndim=3)
-    n_pages, nkv, D = _kv4_pages_of(pages)
-    if page != KV4_PAGE:
-        raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
-    if q.shape[2] != D or q.shape[1] % nkv or q.shape[1] == 0:
+def _kv4_query(q, pages, block_table, step, page: int, scale, softcap, window, keep_first, chunk):
+    """The checks that everything shares that takes queries over a 4-bit cache: (device, sizes, addresses, terms)."""
+    dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
+    qp = _take16(q, "queries", q.dtype, 3, dev)
+    T, nq, d = q.shape
+    if d != D or nq % nkv or nq == 0:
         raise KernelError(f"queries are {tuple(q.shape)} for pages of {nkv} kv heads of {D}")
-    if q.data_ptr() % 16:
-        raise KernelError("queries must start on 16 bytes")
-    _need(block_table, "block table", torch.int32, 2)
-    for t, nm in ((step.slots, "slots"), (step.kv_len, "kv_len"), (step.cu_q, "cu_q")):
-        _need(t, nm, torch.int32, 1)
-    n_seqs = step.slots.shape[0]
-    if step.kv_len.shape[0] != n_seqs or step.cu_q.shape[0] != n_seqs + 1:
+    table = _take(block_table, "block table", _I32, 2, dev)
+    slots, kv_len, cu_q = step.slots, step.kv_len, step.cu_q
+    sl, lens, cu = _take(slots, "slots", _I32, 1, dev), _take(kv_len, "kv_len", _I32, 1, dev), _take(cu_q, "cu_q", _I32, 1, dev)
+    n_seqs = slots.shape[0]
+    if kv_len.shape[0] != n_seqs or cu_q.shape[0] != n_seqs + 1:
         raise KernelError("cu_q, slots and kv_len do not describe one list of sequences")
-    if step.decode and q.shape[0] != n_seqs:
-        raise KernelError(f"{q.shape[0]} rows for {n_seqs} sequences of one token")
-    if (softcap or 0.0) < 0 or (window or 0) < 0 or (keep_first or 0) < 0:
-        raise KernelError("a cap, a window and a number of kept first keys are not negative")
-    _chunk_arg(chunk, keep_first if window else 0)
-    _same_device(q, pages, block_table, step.slots, step.kv_len, step.cu_q)
-    return n_pages, nkv, D
+    if step.decode and T != n_seqs:
+        raise KernelError(f"{T} rows for {n_seqs} sequences of one token")
+    window, softcap, chunk = int(window or 0), float(softcap or 0.0), int(chunk or 0)
+    keep_first = int(keep_first or 0) if window else 0
+    if not (scale > 0 and softcap >= 0 and window >= 0 and keep_first >= 0) or chunk < 0 or (chunk and keep_first):
+        raise KernelError("a scale is positive; a cap, a window, a chunk and a number of kept first keys are not negative, "
+                          "and chunks go without kept first keys")
+    n_slots, max_pages = block_table.shape
+    return dev, (T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, D), (qp, p, table, sl, lens, cu), (
+        window, keep_first, chunk, scale * _LOG2E, softcap * _LOG2E, scale / softcap if softcap else 0.0)
 
 
 def _cost_attention_kv4(out, q, pages, block_table, *, step, window=None, chunk=0, **kw):
     out = out[0] if isinstance(out, tuple) else out
     return _attention_cost(out, q, pages.shape[1] * pages.shape[3] // 16, kv_len=step.kv_len, slots=step.slots,
                            cu_q=step.cu_q, window=window, chunk=chunk)
+
+
+_KV4_ATTN = struct.Struct("@14P13i3f")
+_KV4_PROMPT = struct.Struct("@6P6ifP2f3i")
 
 
 @_profiled("attention_kv4", _cost_attention_kv4)
@@ -1983,78 +1982,66 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     as operands, a prompt with keys and values unpacked to bfloat16), 32-bit queries a 32-bit kernel.  Heads of 64 or
     128 in groups of any size.  ``want_lse``: (out, lse) with lse [T, nq] 32-bit, the natural logarithm of every
     softmax's sum (its sink included; -inf for rows of slot -1, whose output is zeros).  A row that would read a page
-    that there is not comes out as NaN; so does one that sees a token stored as NaN (of a value's, at least the 64
-    elements that are)."""
-    T, nq, _D = q.shape if q.dim() == 3 else (0, 0, 0)
-    keep_first = int(keep_first or 0) if window else 0
-    n_pages, nkv, D = _kv4_query(q, pages, block_table, step, page, softcap, window, keep_first, chunk)
-    _check_sinks(sinks, nq)
-    _same_device(q, sinks)
+    that there is not comes out as NaN, or has more keys than ``step.max_kv_len`` and they do not all fit the launch; so
+    does one that sees a token stored as NaN (of a value's, at least the 64 elements that are)."""
+    dev, sizes, (qp, p, table, sl, lens, cu), (window, keep_first, chunk, scale_log2, cap_log2, cap_inv) = _kv4_query(
+        q, pages, block_table, step, page, scale, softcap, window, keep_first, chunk)
+    T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, D = sizes
+    sk = 0
+    if sinks is not None:
+        sk = _take(sinks, "sinks", _F32, 1, dev)
+        _check_sinks(sinks, nq)
     f32 = _suffix(q.dtype) == "f32"
     out = torch.empty_like(q)
-    lse = torch.empty((T, nq), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((T, nq), dtype=_F32, device=q.device) if want_lse else None
     if T == 0:
         return (out, lse) if want_lse else out
-    n_seqs = step.slots.shape[0]
-    if not step.decode and not f32:
-        a = _AttnTcArgs()
-        a.block_table, a.cu_q, a.slots, a.kv_len = (block_table.data_ptr(), step.cu_q.data_ptr(),
-                                                    step.slots.data_ptr(), step.kv_len.data_ptr())
-        a.out, a.error = out.data_ptr(), _tc_error_flag(q.device).data_ptr()
-        a.n_seqs, a.nq, a.nkv, a.max_pages = n_seqs, nq, nkv, block_table.shape[1]
-        a.pack, rows = prefill_tc_plan(lambda n: _q_blocks(step.q_lens, None, n, T, n_seqs), nq, nkv, _sm_count(q.device))
-        a.n_qblocks = _q_blocks(step.q_lens, None, rows // a.pack, T, n_seqs)
-        while a.n_qblocks > 65535 and a.pack > 1:      # more than a grid has: fewer heads, more tokens a block
-            a.pack //= 2
-            a.n_qblocks = _q_blocks(step.q_lens, None, rows // a.pack, T, n_seqs)
-        a.window, a.scale_log2 = int(window or 0), float(scale) * _LOG2E
-        a.keep_first, a.chunk = keep_first, int(chunk or 0)
-        _set_cap_and_sinks(a, scale, softcap, sinks, nq)
-        with _on(q):
-            _check(_fn("attn_prefill_kv4", "gb_attn_prefill_kv4", "ppppiiiiip")(
-                q.data_ptr(), pages.data_ptr(), ctypes.addressof(a), _ptr(lse), T, n_pages, block_table.shape[0], D, rows,
-                _stream()), "attn_prefill_kv4")
+    lp = lse.data_ptr() if want_lse else 0
+    err = _TC_ERRORS.get(dev)
+    err = (_tc_error_flag(q.device) if err is None else err).data_ptr()
+    sms = _SM_COUNT.get(dev) or _sm_count(q.device)
+    if not (f32 or step.decode):
+        pack, rows = prefill_tc_plan(lambda n: _q_blocks(step.q_lens, None, n, T, n_seqs), nq, nkv, sms)
+        blocks = _q_blocks(step.q_lens, None, rows // pack, T, n_seqs)
+        while blocks > 65535 and pack > 1:      # more than a grid has: fewer heads, more tokens a block
+            pack //= 2
+            blocks = _q_blocks(step.q_lens, None, rows // pack, T, n_seqs)
+        args = _KV4_PROMPT.pack(table, cu, sl, lens, out.data_ptr(), err, n_seqs, nq, nkv, max_pages, window, blocks,
+                                scale_log2, sk, cap_log2, cap_inv, keep_first, chunk, pack)
+        _launch(dev, "attn_prefill_kv4", 1, _fn("attn_prefill_kv4", "gb_attn_prefill_kv4", "ppppiiiiip"), qp, p, args, lp, T,
+                n_pages, n_slots, D, rows)
         return (out, lse) if want_lse else out
-    a = _Kv4AttnArgs()
+    seq = 0
     if not step.decode:
-        _need(step.token_seq, "token_seq", torch.int32, 1)
+        seq = _take(step.token_seq, "token_seq", _I32, 1, dev)
         if step.token_seq.shape[0] != T:
             raise KernelError(f"token_seq has {step.token_seq.shape[0]} entries for {T} rows")
-        a.row_seq = step.token_seq.data_ptr()
-    per = 4 if f32 else 8
-    groups = nkv * ((nq // nkv + per - 1) // per)
-    keys = _keys_visited(step.max_kv_len, window, page, keep_first, int(chunk or 0))
+    each = 4 if f32 else 8
+    groups = nkv * ((nq // nkv + each - 1) // each)
+    keys = _keys_visited(step.max_kv_len, window, page, keep_first, chunk)
+    blocks = 0
     if f32:
-        ns, a.per = kv4_split_plan_f32(T * groups, keys, _sm_count(q.device))
+        ns, per = kv4_split_plan_f32(T * groups, keys, sms)
     else:
-        ns, a.per, blocks = kv4_split_plan(n_seqs, n_seqs * groups, keys, block_table.shape[1], _sm_count(q.device))
-        a.shared = int(blocks > 0)
+        ns, per, blocks = kv4_split_plan(n_seqs, n_seqs * groups, keys, max_pages, sms)
+    po = pm = pc = 0
     if ns > 1:       # (memory of this call's own: two captured graphs, or two streams, share none of it)
-        part = torch.empty(T * nq * ns * (D + 2) + T * groups, dtype=torch.float32, device=q.device)
-        a.part_o, a.part_ml = part.data_ptr(), part.data_ptr() + 4 * T * nq * ns * D
-        a.pieces = part.data_ptr() + 4 * T * nq * ns * (D + 2)
-    a.q, a.pages, a.block_table, a.slots = q.data_ptr(), pages.data_ptr(), block_table.data_ptr(), step.slots.data_ptr()
-    a.kv_len, a.cu_q, a.out, a.lse = step.kv_len.data_ptr(), step.cu_q.data_ptr(), out.data_ptr(), _ptr(lse)
-    a.error = _tc_error_flag(q.device).data_ptr()
-    a.n_rows, a.n_seqs, a.n_slots, a.nq, a.nkv = T, n_seqs, block_table.shape[0], nq, nkv
-    a.max_pages, a.n_pages, a.window, a.n_splits = block_table.shape[1], n_pages, int(window or 0), ns
-    a.keep_first, a.chunk, a.scale_log2 = keep_first, int(chunk or 0), float(scale) * _LOG2E
-    _set_cap_and_sinks(a, scale, softcap, sinks, nq)
-    with _on(q):
-        if f32:
-            _check(_fn("attn_kv4", "gb_attn_kv4_f32", "pip")(ctypes.addressof(a), D, _stream()), "attn_kv4_f32",
-                   2 if ns > 1 else 1)
-        else:
-            _check(_fn("attn_kv4", "gb_attn_kv4_decode", "piip")(ctypes.addressof(a), D, blocks, _stream()),
-                   "attn_kv4_decode", 2 if ns > 1 else 1)
+        n = T * nq * ns
+        part = torch.empty(n * (D + 2) + T * groups, dtype=_F32, device=q.device)
+        po = part.data_ptr()
+        pm = po + 4 * n * D
+        pc = pm + 8 * n
+    args = _KV4_ATTN.pack(qp, p, table, sl, lens, seq, cu, out.data_ptr(), lp, po, pm, pc, err, sk, T, n_seqs, n_slots, nq,
+                          nkv, max_pages, n_pages, window, ns, per, blocks > 0, keep_first, chunk, scale_log2, cap_log2,
+                          cap_inv)
+    if f32:
+        _launch(dev, "attn_kv4_f32", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
+    else:
+        _launch(dev, "attn_kv4_decode", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, blocks)
     return (out, lse) if want_lse else out
 
 
-class _Kv4WeighArgs(ctypes.Structure):
-    _fields_ = [("q", _P), ("lse", _P), ("pages", _P), ("weights", _P), ("block_table", _P), ("slots", _P),
-                ("kv_len", _P), ("cu_q", _P), ("n_rows", _I), ("n_seqs", _I), ("n_slots", _I), ("nq", _I), ("nkv", _I),
-                ("max_pages", _I), ("n_pages", _I), ("window", _I), ("keep_first", _I), ("chunk", _I), ("last", _I),
-                ("scale_log2", _F), ("cap_log2", _F), ("cap_inv", _F)]
+_KV4_WEIGH = struct.Struct("@8P11i3f")
 
 
 @_profiled("kv4_weigh", lambda out, q, lse, *a, **k: (_nbytes(q, lse), 0))
@@ -2063,46 +2050,27 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
               keep_first: int = 0, chunk: int = 0, last: int = 0) -> None:
     """Adds to every cached token's weight, ``weights`` [pages, kv heads, 64] (32-bit, zeros to begin with), the
     attention that the step's queries pay it: the sum over the sequence's rows, or its ``last`` ones, and over the kv
-    head's query heads of exp(score - lse), with the queries and the ``lse`` [T, nq] of ``attention_kv4`` and the
-    arguments that it was called with.  (With prompts' lse a weight is exact to the bfloat16 rounding of the keys that
-    they were computed with.)  A sequence must not appear twice in a step."""
-    keep_first = int(keep_first or 0) if window else 0
-    n_pages, nkv, D = _kv4_query(q, pages, block_table, step, page, softcap, window, keep_first, chunk)
-    if q.dtype != torch.bfloat16:
+    head's query heads of exp(score - lse), with the bfloat16 queries and the ``lse`` [T, nq] of ``attention_kv4`` and
+    the arguments that it was called with.  (With prompts' lse a weight is exact to the bfloat16 rounding of the keys
+    that they were computed with.)  A sequence must not appear twice in a step."""
+    dev, sizes, (qp, p, table, sl, lens, cu), (window, keep_first, chunk, scale_log2, cap_log2, cap_inv) = _kv4_query(
+        q, pages, block_table, step, page, scale, softcap, window, keep_first, chunk)
+    T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, D = sizes
+    if q.dtype is not _BF16:
         raise KernelError(f"weights are gathered from bfloat16 queries, not {q.dtype}")
-    T, nq, _D = q.shape
-    _need(lse, "lse", torch.float32, 2)
-    if tuple(lse.shape) != (T, nq):
+    lp = _take(lse, "lse", _F32, 2, dev)
+    if lse.shape != (T, nq):
         raise KernelError(f"lse is {tuple(lse.shape)}, expected {(T, nq)}")
-    _check_kv4_weights(weights, pages)
-    _same_device(q, lse, weights)
+    w = _take_weights(weights, n_pages, nkv, dev)
     if int(last) < 0:
         raise KernelError("the number of last rows is not negative")
-    a = _Kv4WeighArgs()
-    a.q, a.lse, a.pages, a.weights = q.data_ptr(), lse.data_ptr(), pages.data_ptr(), weights.data_ptr()
-    a.block_table, a.slots = block_table.data_ptr(), step.slots.data_ptr()
-    a.kv_len, a.cu_q = step.kv_len.data_ptr(), step.cu_q.data_ptr()
-    a.n_rows, a.n_seqs, a.n_slots, a.nq, a.nkv = T, step.slots.shape[0], block_table.shape[0], nq, nkv
-    a.max_pages, a.n_pages, a.window, a.last = block_table.shape[1], n_pages, int(window or 0), int(last)
-    a.keep_first, a.chunk, a.scale_log2 = keep_first, int(chunk or 0), float(scale) * _LOG2E
-    a.cap_log2 = float(softcap) * _LOG2E if softcap else 0.0
-    a.cap_inv = float(scale) / float(softcap) if softcap else 0.0
-    blocks = max(1, (step.max_kv_len + KV4_PAGE - 1) // KV4_PAGE)
-    with _on(q):
-        _check(_fn("attn_kv4", "gb_kv4_weigh", "piip")(ctypes.addressof(a), D, min(blocks, 65535), _stream()), "kv4_weigh",
-               1 if T else 0)
+    blocks = min(65535, max(1, (step.max_kv_len + KV4_PAGE - 1) // KV4_PAGE))
+    args = _KV4_WEIGH.pack(qp, lp, p, w, table, sl, lens, cu, T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window,
+                           keep_first, chunk, int(last), scale_log2, cap_log2, cap_inv)
+    _launch(dev, "kv4_weigh", 1 if T else 0, _fn("attn_kv4", "gb_kv4_weigh", "piip"), args, D, blocks)
 
 
-class _Kv4ChooseArgs(ctypes.Structure):
-    _fields_ = [("weights", _P), ("block_table", _P), ("slots", _P), ("kv_len", _P), ("kept", _P), ("new_len", _P),
-                ("n_seqs", _I), ("n_slots", _I), ("nkv", _I), ("max_pages", _I), ("n_pages", _I), ("keep", _I),
-                ("recent", _I), ("first", _I)]
-
-
-class _Kv4MoveArgs(ctypes.Structure):
-    _fields_ = [("src", _P), ("to", _P), ("w_src", _P), ("w_to", _P), ("src_table", _P), ("to_table", _P),
-                ("slots", _P), ("kept", _P), ("n_seqs", _I), ("n_slots", _I), ("nkv", _I), ("n_pages", _I), ("keep", _I),
-                ("src_max", _I), ("to_max", _I), ("in_order", _I)]
+_KV4_CHOOSE, _KV4_MOVE = struct.Struct("@6P8i"), struct.Struct("@8P8i")
 
 
 @_profiled("kv4_evict", lambda out, pages, *a, **k: (2 * out[0].numel() * (pages.shape[3] // 16 + 4), 0))
@@ -2117,54 +2085,41 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     int32 [sequences]).  Sequences of slot -1 keep nothing, shorter ones all they have.  ``into``: a block table like
     ``block_table`` whose pages take the kept tokens (pages that no sequence of the call reads from); without it they
     stay in the sequence's first pages.  A slot must not appear twice."""
-    n_pages, nkv, D = _kv4_pages_of(pages)
-    if page != KV4_PAGE:
-        raise KernelError(f"a cache in 4 bits has pages of {KV4_PAGE} tokens, not {page}")
-    _check_kv4_weights(weights, pages)
-    _need(block_table, "block table", torch.int32, 2)
-    for t, nm in ((slots, "slots"), (kv_len, "kv_len")):
-        _need(t, nm, torch.int32, 1)
+    dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
+    w = _take_weights(weights, n_pages, nkv, dev)
+    table = _take(block_table, "block table", _I32, 2, dev)
+    sl, lens = _take(slots, "slots", _I32, 1, dev), _take(kv_len, "kv_len", _I32, 1, dev)
     n_seqs, keep, recent, first = slots.shape[0], int(keep), int(recent), int(first)
     if kv_len.shape[0] != n_seqs:
         raise KernelError(f"{n_seqs} slots with {kv_len.shape[0]} lengths")
     if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
         raise KernelError(f"{first} first and {recent} recent tokens do not fit {keep} that are kept")
+    n_slots, max_pages = block_table.shape
+    to_table, to_max = table, max_pages
     if into is not None:
-        _need(into, "block table of the kept tokens", torch.int32, 2)
-        if into.shape[0] != block_table.shape[0] or into.shape[1] * KV4_PAGE < min(keep, block_table.shape[1] * KV4_PAGE):
+        to_table, to_max = _take(into, "block table of the kept tokens", _I32, 2, dev), into.shape[1]
+        if into.shape[0] != n_slots or to_max * KV4_PAGE < min(keep, max_pages * KV4_PAGE):
             raise KernelError(f"the block table of the kept tokens is {tuple(into.shape)} for {keep} tokens of "
-                              f"{block_table.shape[0]} slots")
-    _same_device(pages, weights, block_table, slots, kv_len, into)
-    kept = torch.empty((n_seqs, nkv, keep), dtype=torch.int32, device=pages.device)
-    lens = torch.empty((n_seqs,), dtype=torch.int32, device=pages.device)
+                              f"{n_slots} slots")
+    kept = torch.empty((n_seqs, nkv, keep), dtype=_I32, device=pages.device)
+    new = torch.empty((n_seqs,), dtype=_I32, device=pages.device)
     if n_seqs == 0:
-        return kept, lens
-    c = _Kv4ChooseArgs()
-    c.weights, c.block_table, c.slots, c.kv_len = weights.data_ptr(), block_table.data_ptr(), slots.data_ptr(), kv_len.data_ptr()
-    c.kept, c.new_len, c.n_seqs, c.n_slots, c.nkv = kept.data_ptr(), lens.data_ptr(), n_seqs, block_table.shape[0], nkv
-    c.max_pages, c.n_pages, c.keep, c.recent, c.first = block_table.shape[1], n_pages, keep, recent, first
-    m = _Kv4MoveArgs()
-    m.slots, m.kept, m.n_seqs, m.n_slots, m.nkv, m.n_pages, m.keep = (slots.data_ptr(), kept.data_ptr(), n_seqs,
-                                                                     block_table.shape[0], nkv, n_pages, keep)
-    m.src, m.w_src, m.src_table, m.src_max = pages.data_ptr(), weights.data_ptr(), block_table.data_ptr(), block_table.shape[1]
-    m.to, m.w_to = pages.data_ptr(), weights.data_ptr()
-    in_place = into is None or into.data_ptr() == block_table.data_ptr()
-    with _on(pages):
-        _check(_fn("kv4_cache", "gb_kv4_choose", "pp")(ctypes.addressof(c), _stream()), "kv4_choose")
-        move = _fn("kv4_cache", "gb_kv4_move", "pip")
-        if in_place:      # by way of memory of this call's own: tokens move within the pages that others are read from
-            records = (keep + 15) // 16
-            held = torch.empty((n_seqs, nkv, records, pages.shape[3]), dtype=torch.uint8, device=pages.device)
-            w_held = torch.empty((n_seqs, nkv, records * 16), dtype=torch.float32, device=pages.device)
-            m.to, m.w_to, m.to_table = held.data_ptr(), w_held.data_ptr(), None
-            _check(move(ctypes.addressof(m), D, _stream()), "kv4_move")
-            m.src, m.w_src, m.src_table, m.in_order = held.data_ptr(), w_held.data_ptr(), None, 1
-            m.to, m.w_to = pages.data_ptr(), weights.data_ptr()
-            m.to_table, m.to_max = block_table.data_ptr(), block_table.shape[1]
-        else:
-            m.to_table, m.to_max = into.data_ptr(), into.shape[1]
-        _check(move(ctypes.addressof(m), D, _stream()), "kv4_move")
-    return kept, lens
+        return kept, new
+    choose = _KV4_CHOOSE.pack(w, table, sl, lens, kept.data_ptr(), new.data_ptr(), n_seqs, n_slots, nkv, max_pages, n_pages,
+                              keep, recent, first)
+    rest = (sl, kept.data_ptr(), n_seqs, n_slots, nkv, n_pages, keep)
+    evict = _fn("kv4_cache", "gb_kv4_evict", "pppip")
+    if to_table != table:
+        _launch(dev, "kv4_evict", 2, evict, choose, _KV4_MOVE.pack(p, p, w, w, table, to_table, *rest, max_pages, to_max, 0),
+                None, D)
+    else:      # by way of memory of this call's own: tokens move within the pages that others are read from
+        records = (keep + 15) // 16
+        held = torch.empty((n_seqs, nkv, records, pages.shape[3]), dtype=torch.uint8, device=pages.device)
+        w_held = torch.empty((n_seqs, nkv, records * 16), dtype=_F32, device=pages.device)
+        h, wh = held.data_ptr(), w_held.data_ptr()
+        _launch(dev, "kv4_evict", 3, evict, choose, _KV4_MOVE.pack(p, h, w, wh, table, 0, *rest, max_pages, 0, 0),
+                _KV4_MOVE.pack(h, p, wh, w, 0, table, *rest, 0, max_pages, 1), D)
+    return kept, new
 
 
 # ---------------------------------------------------------------- differential attention
