@@ -25,7 +25,7 @@ struct Kv4AttnArgs {
   const float* sinks;      // [nq] one more logit of every head's denominator, or null
   int n_rows, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window, n_splits;
   int per;                 // stretches of 32 keys of a split; shared out: that a block takes at least
-  int shared;              // the blocks share the stretches out evenly
+  int shared;              // 1: the blocks share the stretches out evenly; 2: a pair's splits are a cluster that merges them
   int keep_first, chunk;
   float scale_log2;
   ScoreCap cap;
@@ -134,7 +134,7 @@ struct Kv4Decode {
   // The warps' results: 8 heads each, a head's elements in the order (word's element, lane group) under a pitch that
   // puts a store's 32 lanes into 32 banks.
   static constexpr int PITCH = D + 4;
-  static constexpr int MERGE = WARPS * 8 * (PITCH + 2) * 4;
+  static constexpr int MERGE = WARPS * 8 * (PITCH + 3) * 4 + 64;
   static constexpr int SMEM = RING + MERGE + 128;
 };
 
@@ -293,6 +293,26 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // below 2^8, so it stays below 2^15 and what it loses at the other end is below 2^-25 of a whole probability.  Values
 // are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range; m + 8 s times P
 // is summed in 32 bits.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A number in the shared memory of block `rank` of the cluster, at the same place as here.
+__device__ __forceinline__ float cluster_read(const float* here, int rank) {
+  uint32_t at;
+  float x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(here)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+
+// Element d of a row's head from its maximum, sum and accumulator: the sink joins, and the quotient is stored.
+__device__ __forceinline__ void finish_row(const Kv4AttnArgs& a, int seq, int h, int d, int D, float M, float L, float O) {
+  const size_t row = (size_t)seq * a.nq + h;
+  if (a.sinks && (unsigned)a.slots[seq] < (unsigned)a.n_slots && a.sinks[h] != -INFINITY) O *= add_sink(a.sinks[h], M, L);
+  reinterpret_cast<bf16*>(a.out)[row * D + d] = __float2bfloat16(L != 0.f ? O / L : 0.f);
+  if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
 // A block's part of a pair, for all its threads.
 struct Kv4Part {
   int seq, group, piece, n_pieces;
@@ -328,7 +348,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
   unsigned at = 0, end = 0, run = 1;
   int seq_next = blockIdx.x / (groups * a.n_splits);
   bool more = true;
-  if (a.shared) {
+  if (a.shared == 1) {
     run = share_out(a, C::UNIT, groups, before);
     at = run * blockIdx.x;
     end = min(at + run, (unsigned)before[a.n_seqs] * groups);
@@ -378,7 +398,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     const int slot = live ? a.slots[part.seq] : 0;
     const Stretches list(pos, C::UNIT, BOUNDED ? a.window : 0, BOUNDED ? a.keep_first : 0, BOUNDED ? a.chunk : 0);
     int v_begin;
-    if (a.shared) {
+    if (a.shared == 1) {
       const unsigned first = (unsigned)before[part.seq] * groups, n = (unsigned)list.n;
       part.group = (int)((at - first) / n);
       const unsigned pair = first + part.group * n, piece0 = pair / run;
@@ -402,7 +422,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     lo = list.lo, gap_at = list.n_kept, gap = list.first - list.n_kept;
     table = a.block_table + (size_t)slot * a.max_pages;
     head = a.pages + (size_t)(part.group / hgroups) * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
-    lost = false;
+    lost = a.n_splits > 1 && part.n_pieces > a.n_splits;   // (keys beyond the caller's bound of the lengths)
     asked = 0;
     int page[C::STAGES + 1];
 #pragma unroll
@@ -421,9 +441,12 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
   const bool capped = a.cap.cap_log2 != 0.f;
   float* red_o = reinterpret_cast<float*>(smem + C::RING);     // [warps][8][PITCH]
   float* red_ml = red_o + C::WARPS * 8 * C::PITCH;             // [warps][8][2]
+  float* red_f = red_ml + C::WARPS * 8 * 2;                    // [warps][8]
+  float2* red_h = reinterpret_cast<float2*>(red_f + C::WARPS * 8);     // [8]
 
   Kv4Part part = begin();
-  if (part.piece > 0 && part.piece >= part.n_pieces) return;   // (a split without keys: nothing has been asked for)
+  // (a split without keys has asked for nothing; of a cluster it stays for the others)
+  if (a.shared != 2 && part.piece > 0 && part.piece >= part.n_pieces) return;
   for (;;) {
     Kv4Query<D> q;
     {
@@ -614,29 +637,59 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     __syncthreads();
     const Kv4Part done = part_s[turn_of ^ 1];
     const int h0 = done.group / hgroups * G + done.group % hgroups * 8, heads = min(8, G - done.group % hgroups * 8);
-    const bool alone = done.n_pieces <= 1;             // the result is final
-    const bool live = (unsigned)a.slots[done.seq] < (unsigned)a.n_slots;
-    for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
-      const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
-      float M = -INFINITY;
+    // the warps' share of each head, and the head's maximum and sum
+    if (threadIdx.x < 8) {
+      float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, red_ml[(w * 8 + h) * 2]);
-      float L = 0.f, O = 0.f;
+      for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, red_ml[(w * 8 + threadIdx.x) * 2]);
 #pragma unroll
       for (int w = 0; w < C::WARPS; ++w) {
-        const float mw = red_ml[(w * 8 + h) * 2];
-        const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
-        L += red_ml[(w * 8 + h) * 2 + 1] * f;
-        O += red_o[(w * 8 + h) * C::PITCH + place] * f;
+        const float mw = red_ml[(w * 8 + threadIdx.x) * 2], f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+        L += red_ml[(w * 8 + threadIdx.x) * 2 + 1] * f;
+        red_f[w * 8 + threadIdx.x] = f;
       }
-      const size_t row = (size_t)done.seq * a.nq + h0 + h;
+      red_h[threadIdx.x] = make_float2(M, L);
+    }
+    __syncthreads();
+    const bool alone = done.n_pieces <= 1;             // the result is final
+    if (a.shared == 2) {
+      // The splits of a pair are a cluster: each leaves its sums in its shared memory and finishes a share of the pair's
+      // elements from all of them.
+      for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
+        const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
+        float O = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::WARPS; ++w) O += red_o[(w * 8 + h) * C::PITCH + place] * red_f[w * 8 + h];
+        reinterpret_cast<float*>(smem)[i] = O;         // (the ring is done with)
+      }
+      cluster_barrier();
+      const int n = a.n_splits;
+      for (int i = threadIdx.x * n + done.piece; i < heads * D; i += C::WARPS * 32 * n) {
+        const int h = i / D, d = i % D;
+        float M = -INFINITY, L = 0.f, O = 0.f;
+        for (int c = 0; c < n; ++c) M = fmaxf(M, cluster_read(&red_h[h].x, c));
+        for (int c = 0; c < n; ++c) {
+          const float mc = cluster_read(&red_h[h].x, c), f = mc == -INFINITY ? 0.f : exp2f(mc - M);
+          L += cluster_read(&red_h[h].y, c) * f;
+          O += cluster_read(reinterpret_cast<float*>(smem) + i, c) * f;
+        }
+        finish_row(a, done.seq, h0 + h, d, D, M, L, O);
+      }
+      cluster_barrier();                               // (nobody leaves while its sums are read)
+      break;
+    }
+    for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
+      const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
+      float O = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::WARPS; ++w) O += red_o[(w * 8 + h) * C::PITCH + place] * red_f[w * 8 + h];
+      const float2 ml = red_h[h];
       if (alone) {
-        if (a.sinks && live && a.sinks[h0 + h] != -INFINITY) O *= add_sink(a.sinks[h0 + h], M, L);
-        reinterpret_cast<bf16*>(a.out)[row * D + d] = __float2bfloat16(L != 0.f ? O / L : 0.f);
-        if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+        finish_row(a, done.seq, h0 + h, d, D, ml.x, ml.y, O);
       } else if (done.piece < a.n_splits) {            // (more than the caller's bound of the lengths allows: merged as NaN)
+        const size_t row = (size_t)done.seq * a.nq + h0 + h;
         a.part_o[(row * a.n_splits + done.piece) * D + d] = O;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.n_splits + done.piece) * 2) = make_float2(M, L);
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.n_splits + done.piece) * 2) = ml;
       }
     }
     if (a.n_splits > 1 && done.piece == 0 && threadIdx.x == 0) a.pieces[done.seq * groups + done.group] = done.n_pieces;
@@ -879,69 +932,97 @@ struct Kv4WeighArgs {
 
 #define WEIGH_WARPS 4
 
-// weights[j] += the sum over the sequence's last rows and the kv head's query heads of 2^(s_j c - lse): a warp owns a
-// record of a kv head of a sequence, takes its keys into registers once and adds row after row, head after head, in
-// that order; nobody else touches the record's weights.
+// weights[j] += the sum over the sequence's last rows and the kv head's query heads of 2^(s_j c - lse).  The (row, head)
+// pairs are the columns of the products, eight at a time; a warp has a page of 64 tokens of one kv head, whose keys it
+// asks for all at once, and adds the sums of one set of columns after the other to its tokens' weights: nobody else
+// touches them, and the order is always the same.
 template <int D>
 __global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4WeighArgs a) {
   using F = Kv4<D>;
-  constexpr int NG = F::NG;
+  constexpr int NG = F::NG, NR = KV4_PAGE / KV4_TOKENS;
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, seq = blockIdx.z, G = a.nq / a.nkv;
-  const int slot = a.slots[seq];
-  if ((unsigned)slot >= (unsigned)a.n_slots) return;
+  const int slot = a.slots[seq], len = a.kv_len[seq];
   const int row1 = a.cu_q[seq + 1], row_first = a.cu_q[seq];
+  const int n_pages = (int)min((len + (long long)KV4_PAGE - 1) / KV4_PAGE, (long long)a.max_pages);
+  int tile = blockIdx.x * WEIGH_WARPS + warp;
+  if ((unsigned)slot >= (unsigned)a.n_slots || tile >= n_pages) return;
   const int row0 = a.last > 0 ? max(row_first, row1 - a.last) : row_first;
   if (row0 >= row1 || row_first < 0 || row1 > a.n_rows) return;
-  const int len = a.kv_len[seq];
   const int pos0 = len - (row1 - row0);                          // the position of row0
   const int* table = a.block_table + (size_t)slot * a.max_pages;
   const int lowest = first_key(max(pos0, 0), a.window, a.chunk);  // no row sees a key below it but for the kept ones
   const int keep = a.window > 0 ? a.keep_first : 0;
-  const int records = (len + KV4_TOKENS - 1) / KV4_TOKENS;
   const uint32_t magic = kv4_magic(a.n_seqs);
-  for (int rec = blockIdx.x * WEIGH_WARPS + warp; rec < records; rec += gridDim.x * WEIGH_WARPS) {
-    const int key0 = rec * KV4_TOKENS;
-    if (key0 + KV4_TOKENS <= lowest && key0 >= keep) continue;
-    const int page = kv4_page(table, key0 / KV4_PAGE, a.max_pages, a.n_pages);
+  const int tok = kv4_token(r), columns = (row1 - row0) * G;
+  const bool capped = a.cap.cap_log2 != 0.f;
+  // column c is head c % G of row c / G; this lane loads the query of column r of a set and sums columns 2 t, 2 t + 1
+  auto query = [&](int c) {
+    return c < columns ? a.q + ((size_t)(row0 + c / G) * a.nq + kvh * G + c % G) * D : nullptr;
+  };
+  Kv4Query<D> q;
+  q.load(query(r));
+  for (; tile < n_pages; tile += gridDim.x * WEIGH_WARPS) {
+    const int key0 = tile * KV4_PAGE;
+    if (key0 + KV4_PAGE <= lowest && key0 >= keep) continue;
+    const int page = kv4_page(table, tile, a.max_pages, a.n_pages);
     if (page < 0) continue;
     const size_t at = (size_t)page * a.nkv + kvh;
-    const uint8_t* b = a.pages + (at * (KV4_PAGE / KV4_TOKENS) + (rec & 3)) * F::RECORD;
-    const int tok = kv4_token(r), ja = key0 + tok, jb = ja + 8;
-    uint32_t ka[D / 32], kb[D / 32], pa[2 * NG], pb[2 * NG];
-    load_words(b + tok * F::ROW + t * (D / 8), ka);
-    load_words(b + (tok + 8) * F::ROW + t * (D / 8), kb);
-    load_words(b + F::PAIR_OFF + tok * F::PAIR, pa);
-    load_words(b + F::PAIR_OFF + (tok + 8) * F::PAIR, pb);
-    float wa = 0.f, wb = 0.f;
-    for (int row = row0; row < row1; ++row) {
-      const int pos = pos0 + row - row0, lo = first_key(max(pos, 0), a.window, a.chunk);
-      const bool see_a = ja <= pos && (ja >= lo || ja < keep), see_b = jb <= pos && (jb >= lo || jb < keep);
-      if (!__any_sync(0xffffffffu, see_a || see_b)) continue;
-      for (int hc = 0; hc < G; hc += 8) {
-        const int h0 = kvh * G + hc, heads = min(8, G - hc);
-        Kv4Query<D> q;
-        float s[4];
-        q.load(r < heads ? a.q + ((size_t)row * a.nq + h0 + r) * D : nullptr);
-        kv4_scores<D>(ka, kb, pa, pb, q, magic, s);
+    uint32_t ka[NR][D / 32], kb[NR][D / 32], pa[NR][NG], pb[NR][NG];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float lse = 2 * t + i < heads ? a.lse[(size_t)row * a.nq + h0 + 2 * t + i] * 1.4426950408889634f : -INFINITY;
+    for (int u = 0; u < NR; ++u) {
+      const uint8_t* b = a.pages + (at * NR + u) * F::RECORD;
+      load_words(b + tok * F::ROW + t * (D / 8), ka[u]);
+      load_words(b + (tok + 8) * F::ROW + t * (D / 8), kb[u]);
+      load_words(b + F::PAIR_OFF + tok * F::PAIR, pa[u]);
+      load_words(b + F::PAIR_OFF + (tok + 8) * F::PAIR, pb[u]);
+    }
+    float* w = a.weights + at * KV4_PAGE;
+    float sum[NR][2];
+#pragma unroll
+    for (int u = 0; u < NR; ++u) sum[u][0] = sum[u][1] = 0.f;
+    for (int c0 = 0; c0 < columns; c0 += 8) {
+      if (columns > 8) q.load(query(c0 + r));
+      // what this lane's two columns see, and their factors
+      int last[2], first[2];
+      float lse[2], factor[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = c0 + 2 * t + i, row = row0 + c / G;
+        last[i] = -1, first[i] = 0, lse[i] = 0.f;
+        if (c < columns) {
+          lse[i] = a.lse[(size_t)row * a.nq + kvh * G + c % G] * 1.4426950408889634f;
+          if (lse[i] != -INFINITY) last[i] = pos0 + row - row0, first[i] = first_key(max(last[i], 0), a.window, a.chunk);
+        }
+        factor[i] = (capped ? a.cap.cap_inv : a.scale_log2) * q.back[i];
+      }
+#pragma unroll
+      for (int u = 0; u < NR; ++u) {
+        float s[4];
+        kv4_scores<D>(ka[u], kb[u], pa[u], pb[u], q, magic, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float x = s[2 * half + i] * q.back[i];
-            const float y = a.cap.cap_log2 != 0.f ? capped_log2(x * a.cap.cap_inv, a.cap) : x * a.scale_log2;
-            if (lse != -INFINITY && (half ? see_b : see_a)) (half ? wb : wa) += exp2f(y - lse);
+            const int j = key0 + u * KV4_TOKENS + tok + half * 8;
+            float x = s[2 * half + i] * factor[i];
+            if (capped) x = capped_log2(x, a.cap);
+            const float p = exp2_fast(x - lse[i]);
+            if (j <= last[i] && (j >= first[i] || j < keep)) sum[u][half] += p;
           }
-        }
       }
     }
-    wa += __shfl_xor_sync(0xffffffffu, wa, 1), wb += __shfl_xor_sync(0xffffffffu, wb, 1);
-    wa += __shfl_xor_sync(0xffffffffu, wa, 2), wb += __shfl_xor_sync(0xffffffffu, wb, 2);
-    float* w = a.weights + at * KV4_PAGE + (key0 & (KV4_PAGE - 1));
-    if (t == 0 && ja < len) w[tok] += wa;
-    if (t == 1 && jb < len) w[tok + 8] += wb;
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 1);
+        sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 2);
+        // (a lane of each row's four has a record's two tokens)
+        const int j = u * KV4_TOKENS + tok + half * 8;
+        if (t == u && key0 + j < len) w[j] += sum[u][half];
+      }
   }
 }
 
@@ -952,7 +1033,7 @@ static int checked(const Kv4AttnArgs* a, int D) {
       a->nq <= 0 || a->nkv <= 0 || a->nq % a->nkv || a->max_pages <= 0 || a->max_pages > 0x1000000 || a->n_pages <= 0 || a->n_slots < 0 ||
       a->n_splits <= 0 || a->per <= 0 || a->chunk < 0 || a->window < 0 || a->keep_first < 0)
     return GB_ERR_BAD_ARG;
-  if (a->n_splits > 1 && (!a->part_o || !a->part_ml || !a->pieces)) return GB_ERR_BAD_ARG;
+  if (a->n_splits > 1 && a->shared != 2 && (!a->part_o || !a->part_ml || !a->pieces)) return GB_ERR_BAD_ARG;
   if (((uintptr_t)a->q | (uintptr_t)a->pages) & 15) return GB_ERR_BAD_ARG;
   return 0;
 }
@@ -968,7 +1049,8 @@ static int decode_launch(const Kv4AttnArgs& a, unsigned grid, cudaStream_t s) {
     if (e != cudaSuccess) return (int)e;
     if (dev < 64) configured[dev] = true;
   }
-  return gb_launch(kv4_decode_kernel<D, BOUNDED>, dim3(grid), dim3(Kv4Decode<D>::WARPS * 32), Kv4Decode<D>::SMEM, s, a);
+  return gb_launch_cluster(kv4_decode_kernel<D, BOUNDED>, dim3(grid), dim3(Kv4Decode<D>::WARPS * 32), Kv4Decode<D>::SMEM, s,
+                           a.shared == 2 ? a.n_splits : 1, a);
 }
 
 template <int D>
@@ -977,16 +1059,17 @@ static int decode(const Kv4AttnArgs& a, int blocks, cudaStream_t s) {
   const long long pairs = (long long)a.nkv * hgroups * a.n_seqs;
   if (pairs * a.n_splits > 0x7fffffffll) return GB_ERR_UNSUPPORTED;
   // (all stretches are counted in 32 bits, and a block's run may reach beyond them)
-  if (a.shared && (a.n_splits < 2 || a.n_seqs > KV4_SHARED_SEQS || blocks <= 0 ||
+  if (a.shared == 2 && (a.n_splits < 2 || a.n_splits > 8)) return GB_ERR_BAD_ARG;
+  if (a.shared == 1 && (a.n_splits < 2 || a.n_seqs > KV4_SHARED_SEQS || blocks <= 0 ||
                    pairs * (4ll * a.max_pages + 4) + 2ll * blocks * a.per > 0x7fffffffll))
     return GB_ERR_BAD_ARG;
-  const unsigned grid = (unsigned)(a.shared ? blocks : pairs * a.n_splits);
+  const unsigned grid = (unsigned)(a.shared == 1 ? blocks : pairs * a.n_splits);
   const int rc = a.window > 0 || a.chunk > 0 ? decode_launch<D, true>(a, grid, s) : decode_launch<D, false>(a, grid, s);
-  if (rc || a.n_splits == 1) return rc;
+  if (rc || a.n_splits == 1 || a.shared == 2) return rc;
   return gb_launch(kv4_merge_kernel<bf16>, dim3((unsigned)(a.n_rows * a.nq)), dim3(D), 0, s, a, D, 8);
 }
 
-// `blocks`: how many share the keys out (a->shared).
+// `blocks`: how many share the keys out (a->shared 1).
 GB_EXPORT int gb_attn_kv4_decode(const Kv4AttnArgs* a, int D, int blocks, cudaStream_t s) {
   const int rc = checked(a, D);
   if (rc) return rc;

@@ -60,26 +60,35 @@ __device__ __forceinline__ void store8<bf16>(bf16* p, const float (&x)[8]) {
 // The bits of the bfloat16 number next to x on the side of larger magnitude (x itself when it is one).
 __device__ __forceinline__ uint32_t bf16_away(float x) { return (__float_as_uint(x) + 0xffffu) >> 16; }
 
+// The code of x - m = d in steps of s: the nearest whole number to d / s, of two equally near ones the even one.  The
+// product with the inverse is off by a few units of its last place, so its whole number can be wrong by one where d / s
+// lies that close to the middle of two; the remainder d - c s, which one multiply-add gives to its last place, says so.
+// (A rounded quotient takes a long way round for d = 0, which every group has: a step's rows of 64 tokens took 11 us.)
+__device__ __forceinline__ uint32_t nearest_code(float d, float s, float inv, float half) {
+  const float c = rintf(d * inv);
+  const float rest = fmaf(-c, s, d);
+  const int k = (int)c, odd = k & 1;
+  const int up = rest > half || (odd && rest == half), down = rest < -half || (odd && rest == -half);
+  return (uint32_t)min(max(k + up - down, 0), 15);
+}
+
 // Eight lanes take a group of 64 elements, a word's eight each: the group's range is three exchanges, its codes and
-// pair are written straight to their places.  A row of codes (64 bytes at D 128) comes from one warp.
+// pair are written straight to their places.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsArgs a) {
   using F = Kv4<D>;
   pdl_wait();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long group = i >> 3;
-  const int lane8 = i & 7;
-  const long long n_groups = (long long)a.T * 2 * a.nkv * F::NG;
-  if (group >= n_groups) return;                       // (whole groups of lanes leave)
+  const unsigned group = blockIdx.x * 32 + (threadIdx.x >> 3), heads = 2 * a.nkv;
+  const int lane8 = threadIdx.x & 7;
+  if (group >= (unsigned)a.T * heads * F::NG) return;          // (whole groups of lanes leave; fits 32 bits)
   const uint32_t mask = 0xffu << (threadIdx.x & 24);
-  const int g = group % F::NG;
-  const long long row = group / F::NG;
-  const int hh = row % (2 * a.nkv), t = row / (2 * a.nkv);
+  const unsigned g = group % F::NG, row = group / F::NG;
+  const int t = row / heads, hh = row - t * heads;
   float x[8];
-  load8(reinterpret_cast<const T*>(a.kv) + row * D + g * KV4_GROUP + lane8 * 8, x);
+  load8(reinterpret_cast<const T*>(a.kv) + (size_t)row * D + g * KV4_GROUP + lane8 * 8, x);
   int place;
   const int page = find_token(a, t, place);
-  if (page < 0) return;                                // (the same for the group's lanes)
+  if (page < 0) return;                                         // (the same for the group's lanes)
   float lo = x[0], hi = x[0];
   bool fine = true;
 #pragma unroll
@@ -95,17 +104,18 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsArgs a) {
   fine = __ballot_sync(mask, fine) == mask;
   const uint32_t mb = lo < 0.f ? bf16_away(lo) : __float_as_uint(lo) >> 16;      // towards minus infinity
   const float m = __uint_as_float(mb << 16);
-  uint32_t sb = bf16_away(__fdiv_rn(__fsub_rn(hi, m), 15.f));                     // upwards: it is not negative
+  const uint32_t sb = bf16_away(__fdiv_rn(__fsub_rn(hi, m), 15.f));               // upwards: it is not negative
   const float s = __uint_as_float(sb << 16);
   uint32_t word = 0, pair = (mb << 16) | sb;
   if (!fine || !isfinite(s) || !isfinite(m)) {
-    pair = 0x7fff7fffu;                                // NaN, NaN
+    pair = 0x7fff7fffu;                                         // NaN, NaN
   } else if (s > 0.f) {
+    // (steps at the ends of the numbers' range are brought to its middle by a power of two, exactly)
+    const float scale = s < 1e-30f ? 0x1p100f : s > 1e30f ? 0x1p-100f : 1.f;
+    const float s1 = s * scale, inv = __fdividef(1.f, s1), half = 0.5f * s1;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t c = (uint32_t)__float2int_rn(__fdiv_rn(__fsub_rn(x[e], m), s));
-      word |= min(c, 15u) << (((e & 1) << 4) + ((e >> 1) << 2));
-    }
+    for (int e = 0; e < 8; ++e)
+      word |= nearest_code(__fsub_rn(x[e], m) * scale, s1, inv, half) << (((e & 1) << 4) + ((e >> 1) << 2));
   }
   const bool is_v = hh >= a.nkv;
   const int h = is_v ? hh - a.nkv : hh, tok = place & (KV4_TOKENS - 1), n = g * 8 + lane8;
@@ -118,41 +128,62 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsArgs a) {
   }
 }
 
-// The same lanes the other way: a word and its pair in, eight elements out (zeros for a token that is nowhere).
+#define ROWS_WARPS 4
+#define ROWS_AT_ONCE 4
+
+// The other way: a word and its pair in, eight elements out (zeros for a token that is nowhere).  A warp has a token,
+// finds once where it lives and has ROWS_AT_ONCE turns' loads on their way together.  (A thread for every word, which
+// found the token for itself by four loads in a row, read 16,384 tokens of 8 heads of 128 in 29.3 us, this in 16.0: 86 MB
+// at 5.4 TB/s.)
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsArgs a) {
+__global__ void __launch_bounds__(32 * ROWS_WARPS) kv4_read_kernel(const Kv4RowsArgs a) {
   using F = Kv4<D>;
   pdl_wait();
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int n = i % (D / 8);
-  const long long row = i / (D / 8);
-  if (row >= (long long)a.T * 2 * a.nkv) return;
-  const int hh = row % (2 * a.nkv), t = row / (2 * a.nkv);
+  const int t = blockIdx.x * ROWS_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= a.T) return;
+  const int words = 2 * a.nkv * (D / 8);
+  T* out = reinterpret_cast<T*>(a.out) + (size_t)t * words * 8;
   int place;
   const int page = find_token(a, t, place);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (page >= 0) {
-    const bool is_v = hh >= a.nkv;
-    const int h = is_v ? hh - a.nkv : hh, tok = place & (KV4_TOKENS - 1);
-    const uint8_t* rec = a.pages + (((size_t)page * a.nkv + h) * (KV4_PAGE / KV4_TOKENS) + place / KV4_TOKENS) * F::RECORD;
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(rec + (is_v ? F::V_OFF : 0) + tok * F::ROW);
-    const uint32_t w = codes[is_v ? F::value_word(n, tok) : F::key_word(n)];
-    const uint32_t pair = reinterpret_cast<const uint32_t*>(rec + F::PAIR_OFF + tok * F::PAIR)[(is_v ? F::NG : 0) + n / 8];
-    const float s = kv4_s(pair), m = kv4_m(pair);
+  const int tok = place & (KV4_TOKENS - 1);
+  const uint8_t* first = a.pages + ((size_t)max(page, 0) * a.nkv * (KV4_PAGE / KV4_TOKENS) + place / KV4_TOKENS) * F::RECORD;
+  for (int i0 = lane; i0 < words; i0 += 32 * ROWS_AT_ONCE) {
+    uint32_t w[ROWS_AT_ONCE], pair[ROWS_AT_ONCE];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)kv4_code(w, e), m);
+    for (int u = 0; u < ROWS_AT_ONCE; ++u) {
+      const int i = i0 + 32 * u, hh = i / (D / 8), n = i % (D / 8);
+      w[u] = pair[u] = 0u;
+      if (i < words && page >= 0) {
+        const bool is_v = hh >= a.nkv;
+        const uint8_t* rec = first + (size_t)(is_v ? hh - a.nkv : hh) * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
+        const uint32_t* codes = reinterpret_cast<const uint32_t*>(rec + (is_v ? F::V_OFF : 0) + tok * F::ROW);
+        w[u] = codes[is_v ? F::value_word(n, tok) : F::key_word(n)];
+        pair[u] = reinterpret_cast<const uint32_t*>(rec + F::PAIR_OFF + tok * F::PAIR)[(is_v ? F::NG : 0) + n / 8];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS_AT_ONCE; ++u) {
+      if (i0 + 32 * u >= words) break;
+      const float s = kv4_s(pair[u]), m = kv4_m(pair[u]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)kv4_code(w[u], e), m);
+      store8(out + (size_t)(i0 + 32 * u) * 8, x);
+    }
   }
-  store8(reinterpret_cast<T*>(a.out) + row * D + n * 8, x);
 }
 
 template <typename T, int D>
 static int launch_rows(const Kv4RowsArgs& a, bool write, cudaStream_t s) {
-  const long long threads = (long long)a.T * 2 * a.nkv * (D / 8), blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffll) return GB_ERR_UNSUPPORTED;
-  return gb_launch(write ? kv4_write_kernel<T, D> : kv4_read_kernel<T, D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+  if (!write)
+    return gb_launch(kv4_read_kernel<T, D>, dim3((a.T + ROWS_WARPS - 1) / ROWS_WARPS), dim3(32 * ROWS_WARPS), 0, s, a);
+  const long long groups = (long long)a.T * 2 * a.nkv * (D / KV4_GROUP), blocks = (groups + 31) / 32;
+  if (groups > 0x7fffffffll) return GB_ERR_UNSUPPORTED;
+  return gb_launch(kv4_write_kernel<T, D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
 }
 static int rows(const Kv4RowsArgs* a, int D, int f32, bool write, cudaStream_t s) {
-  if (a->T < 0 || a->nkv <= 0 || a->max_pages <= 0 || a->n_pages <= 0 || a->n_seqs < 0 || a->n_slots < 0 || !a->pages)
+  if (a->T < 0 || a->nkv <= 0 || a->max_pages <= 0 || a->n_pages <= 0 || a->n_seqs < 0 || a->n_slots < 0 || !a->pages ||
+      a->T > 0x7fffff00 || a->nkv > 0x100000)
     return GB_ERR_BAD_ARG;
   if (((uintptr_t)(write ? a->kv : a->out) | (uintptr_t)a->pages) & 15) return GB_ERR_BAD_ARG;
   if (a->T == 0) return 0;
@@ -182,15 +213,46 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 
 #define CHOOSE_THREADS 1024
+#define CHOOSE_WARPS (CHOOSE_THREADS / 32)
+#define CHOOSE_BINS 2048
+#define CHOOSE_HELD (40 * 1024)      // the most weights that a block holds in shared memory; those behind are read again
 
-// One block chooses for one kv head of one sequence.  The weight of the last token that is kept among the candidates
-// is found digit by digit (four passes over eight bits, a histogram each); one more pass in the order of the tokens
-// then writes the places of the kept ones, with the first of those that are equal to the last one kept.
-__global__ void __launch_bounds__(CHOOSE_THREADS) kv4_choose_kernel(const Kv4ChooseArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum_s[2][32];
-  __shared__ uint32_t digit_s;
-  __shared__ int left_s;
+// A whole block finds the largest digit d for which at least `left` of the counted weights have a digit >= d, and how
+// many are above it: the threads have a few bins each, from the largest down.
+__device__ __forceinline__ void find_digit(const int* hist, int bins, int left, int* warp_sums, int* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = bins / CHOOSE_THREADS;
+  int mine = 0;
+  for (int i = 0; i < each; ++i) mine += hist[bins - 1 - tid * each - i];
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  int before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0) + sum - mine;
+  if (before < left && before + mine >= left) {
+    int i = 0;
+    for (;; ++i) {
+      const int n = hist[bins - 1 - tid * each - i];
+      if (before + n >= left) break;
+      before += n;
+    }
+    found[0] = bins - 1 - tid * each - i, found[1] = left - before;
+  }
+  __syncthreads();
+}
+
+// One block chooses for one kv head of one sequence.  The weights are read once and held in shared memory; the one of
+// the last token that is kept among the candidates is found digit by digit (11, 11 and 10 bits, a histogram each).  Each
+// warp then has a stretch of the tokens: it counts those above that weight and those equal to it, and writes the places
+// of the kept ones behind those of the warps in front of it, with the first of those that are equal to the last kept.
+__global__ void __launch_bounds__(CHOOSE_THREADS) kv4_choose_kernel(const Kv4ChooseArgs a, int held) {
+  extern __shared__ uint32_t held_s[];
+  __shared__ int hist[CHOOSE_BINS];
+  __shared__ int sums[2][CHOOSE_WARPS];
+  __shared__ int found[2];
   pdl_wait();
   const int h = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slot = a.slots[seq];
@@ -207,79 +269,85 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) kv4_choose_kernel(const Kv4Cho
   const int* table = a.block_table + (size_t)slot * a.max_pages;
   const int c0 = a.first, c1 = len - a.recent;          // the candidates; first + recent <= keep < len
   const int need = keep - a.first - a.recent;
-  auto weight = [&](int i) -> uint32_t {
+  auto read = [&](int i) -> uint32_t {
     const int page = kv4_page(table, i / KV4_PAGE, a.max_pages, a.n_pages);
     return page < 0 ? 0u : ordered(a.weights[((size_t)page * a.nkv + h) * KV4_PAGE + (i & (KV4_PAGE - 1))]);
   };
-  uint32_t last = 0xffffffffu;                          // the weight of the last one kept (nothing is above it)
-  int left = 0;                                         // how many of that weight are kept
-  if (need > 0) {
-    last = 0;
-    left = need;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += CHOOSE_THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int i = c0 + tid; i < c1; i += CHOOSE_THREADS) {
-        const uint32_t u = weight(i);
-        if (shift == 24 || (u >> (shift + 8)) == (last >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (warp == 0) {                                  // from the largest digit down: the one where `left` runs out
-        int above = 0;
-        for (int top = 255; top >= 0; top -= 32) {
-          const int n = hist[top - lane];
-          int sum = n;
+  auto weight = [&](int i) -> uint32_t { return i < held ? held_s[i] : read(i); };
+  uint32_t last = 0;                                    // the weight of the last one kept, from its top digit down
+  int left = need;                                      // how many of that weight are kept
+#pragma unroll 1
+  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < bins; i += CHOOSE_THREADS) hist[i] = 0;
+    __syncthreads();
+    if (pass == 0) {
+      for (int i0 = c0 + tid; i0 < c1; i0 += 4 * CHOOSE_THREADS) {      // (four loads on their way at a time)
+        uint32_t u[4];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-          }
-          const uint32_t hit = __ballot_sync(0xffffffffu, above + sum >= left);
-          if (hit) {
-            const int at = __ffs(hit) - 1;
-            const int before = above + __shfl_sync(0xffffffffu, sum - n, at);
-            if (lane == 0) digit_s = (uint32_t)(top - at), left_s = left - before;
-            break;
-          }
-          above += __shfl_sync(0xffffffffu, sum, 31);
+        for (int k = 0; k < 4; ++k) u[k] = i0 + k * CHOOSE_THREADS < c1 ? read(i0 + k * CHOOSE_THREADS) : 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + k * CHOOSE_THREADS;
+          if (i >= c1) break;
+          if (i < held) held_s[i] = u[k];
+          atomicAdd(&hist[u[k] >> 21], 1);
         }
       }
-      __syncthreads();
-      last |= digit_s << shift;
-      left = left_s;
-      __syncthreads();
+    } else {
+      const int done = pass == 1 ? 21 : 10;
+      for (int i = c0 + tid; i < c1; i += CHOOSE_THREADS) {
+        const uint32_t u = weight(i);
+        if (u >> done == last >> done) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1);
+      }
     }
+    __syncthreads();
+    find_digit(hist, bins, left, sums[0], found);
+    last |= (uint32_t)found[0] << shift;
+    left = found[1];
+    __syncthreads();
   }
-  int out = 0, equal = 0;                               // kept, and equal to the last, in front of this stretch
-  for (int base = 0; base < len; base += CHOOSE_THREADS) {
-    const int i = base + tid;
-    const bool in = i < len, sure = in && (i < c0 || i >= c1);
-    const uint32_t u = in && !sure && need > 0 ? weight(i) : 0u;
-    const bool cand = in && !sure && need > 0;
-    const bool tie = cand && u == last;
+  // warp w has tokens [w each, (w + 1) each)
+  const int each = (len + CHOOSE_THREADS - 1) / CHOOSE_THREADS * 32, begin = warp * each, end = min(len, begin + each);
+  auto kind = [&](int i, bool& sure, bool& tie) {       // kept whatever the others are; or equal to the last one kept
+    sure = i < end && (i < c0 || i >= c1);
+    tie = false;
+    if (i < end && !sure && need > 0) {
+      const uint32_t u = weight(i);
+      sure = u > last, tie = u == last;
+    }
+  };
+  int n_sure = 0, n_tie = 0;
+  for (int i = begin + lane; i - lane < end; i += 32) {
+    bool sure, tie;
+    kind(i, sure, tie);
+    n_sure += __popc(__ballot_sync(0xffffffffu, sure)), n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+  }
+  if (lane == 0) sums[0][warp] = n_sure, sums[1][warp] = n_tie;
+  __syncthreads();
+  int ties_before, out;
+  {
+    const int t_all = sums[1][lane], s_all = sums[0][lane];
+    int t_sum = t_all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, t_sum, o);
+      if (lane >= o) t_sum += v;
+    }
+    const int before = t_sum - t_all;                   // of warp `lane`
+    const int taken = s_all + min(max(left - before, 0), t_all);
+    out = __reduce_add_sync(0xffffffffu, lane < warp ? taken : 0);
+    ties_before = __shfl_sync(0xffffffffu, before, warp);
+  }
+  for (int i = begin + lane; i - lane < end; i += 32) {
+    bool sure, tie;
+    kind(i, sure, tie);
     const uint32_t ties = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) warp_sum_s[0][warp] = __popc(ties);
-    __syncthreads();
-    int t_before = 0, t_all = 0;
-    for (int w = 0; w < CHOOSE_THREADS / 32; ++w) {
-      const int n = warp_sum_s[0][w];
-      t_before += w < warp ? n : 0;
-      t_all += n;
-    }
-    const int rank = equal + t_before + __popc(ties & ((1u << lane) - 1));
-    const bool mine = sure || (cand && (u > last || (tie && rank < left)));
+    const bool mine = sure || (tie && ties_before + __popc(ties & ((1u << lane) - 1)) < left);
     const uint32_t who = __ballot_sync(0xffffffffu, mine);
-    if (lane == 0) warp_sum_s[1][warp] = __popc(who);
-    __syncthreads();
-    int k_before = 0, k_all = 0;
-    for (int w = 0; w < CHOOSE_THREADS / 32; ++w) {
-      const int n = warp_sum_s[1][w];
-      k_before += w < warp ? n : 0;
-      k_all += n;
-    }
-    if (mine) kept[out + k_before + __popc(who & ((1u << lane) - 1))] = i;
-    out += k_all;
-    equal += t_all;
+    if (mine) kept[out + __popc(who & ((1u << lane) - 1))] = i;
+    out += __popc(who);
+    ties_before += __popc(ties);
   }
 }
 
@@ -391,7 +459,18 @@ static int choose(const Kv4ChooseArgs* a, cudaStream_t s) {
       a->first < 0 || a->recent < 0 || a->keep <= 0 || a->first > a->keep || a->recent > a->keep - a->first)
     return GB_ERR_BAD_ARG;
   if (a->n_seqs > GB_MAX_GRID_YZ) return GB_ERR_UNSUPPORTED;
-  return gb_launch(kv4_choose_kernel, dim3(a->nkv, a->n_seqs), dim3(CHOOSE_THREADS), 0, s, *a);
+  const long long room = (long long)a->max_pages * KV4_PAGE;
+  const int held = room < CHOOSE_HELD ? (int)room : CHOOSE_HELD;
+  static bool configured[64] = {};     // (the shared-memory size is a property of a kernel on one device)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(kv4_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, CHOOSE_HELD * 4);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 64) configured[dev] = true;
+  }
+  return gb_launch(kv4_choose_kernel, dim3(a->nkv, a->n_seqs), dim3(CHOOSE_THREADS), (size_t)held * 4, s, *a, held);
 }
 
 static int move(const Kv4MoveArgs* a, int D, cudaStream_t s) {

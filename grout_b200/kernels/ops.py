@@ -1904,31 +1904,32 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
     the block table."""
     dev, nkv, D, T, rest = _kv4_rows(pages, None, token_seq, token_pos, slots, block_table, page)
     f32 = _suffix(dtype) == "f32"
-    out = torch.empty((T, 2 * nkv, D), dtype=dtype, device=pages.device)
+    out = pages.new_empty((T, 2 * nkv, D), dtype=dtype)
     _launch(dev, "kv4_read", 1 if T else 0, _fn("kv4_cache", "gb_kv4_read", "piip"),
             _KV4_ROWS.pack(0, out.data_ptr(), *rest), D, f32)
     return out
 
 
 KV4_LEAST = 8              # stretches of 32 keys that a block takes at least (two for each of its warps)
-KV4_WHOLE = 16             # up to so many a block takes all of a pair
 KV4_SPLIT_OVERRIDE: Optional[int] = None      # stretches that a block takes at least, for experiments
-KV4_SHARE_OVERRIDE: Optional[bool] = None     # whether they are shared out, for tests
+KV4_SHARE_OVERRIDE: Optional[int] = None      # how pairs are split (0, 1 or 2, see kv4_split_plan), for tests
 
 
 def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int) -> Tuple[int, int, int]:
-    """(splits, stretches of 32 keys, blocks) of the bfloat16 kernel for ``pairs`` (sequence, group of query heads)
-    pairs of up to ``keys`` keys.  One split: a block a pair.  More and no blocks: a block a split of so many stretches.
-    With blocks: they share the stretches out, at least so many each, and a pair has at most so many of them."""
+    """(splits, stretches of 32 keys in a split, way) of the bfloat16 kernel for ``pairs`` (sequence, group of query
+    heads) pairs of up to ``keys`` keys.  Way 0: a block a split, merged by a second kernel (one split: nothing to
+    merge); 2: the splits of a pair are a cluster of up to eight blocks that merges them; 1: four blocks an SM share all
+    stretches out, at least so many each, and a pair has at most so many splits."""
     tiles = max(1, (keys + 31) // 32)
-    least = KV4_SPLIT_OVERRIDE or (tiles if tiles <= KV4_WHOLE else max(KV4_LEAST, -(-tiles // 62)))
-    if tiles <= least:
+    least = KV4_SPLIT_OVERRIDE or max(KV4_LEAST, -(-tiles // 62))
+    splits, blocks, way = -(-tiles // least), 4 * sms, KV4_SHARE_OVERRIDE
+    if splits == 1:
         return 1, tiles, 0
-    splits, blocks = -(-tiles // least), 4 * sms
-    share = splits * pairs > blocks if KV4_SHARE_OVERRIDE is None else KV4_SHARE_OVERRIDE
-    if share and n_seqs <= 256 and pairs * (4 * max_pages + 4) + 2 * blocks * least <= 0x7fffffff:
-        return min(blocks, splits + 1), least, blocks
-    return splits, least, 0
+    if way is None:
+        way = 1 if splits * pairs > blocks else 2 if splits <= 8 else 0
+    if way == 1 and n_seqs <= 256 and pairs * (4 * max_pages + 4) + 2 * blocks * least <= 0x7fffffff:
+        return min(blocks, splits + 1), least, 1
+    return splits, least, 2 if way == 2 and splits <= 8 else 0
 
 
 def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int]:
@@ -1993,7 +1994,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         _check_sinks(sinks, nq)
     f32 = _suffix(q.dtype) == "f32"
     out = torch.empty_like(q)
-    lse = torch.empty((T, nq), dtype=_F32, device=q.device) if want_lse else None
+    lse = q.new_empty((T, nq), dtype=_F32) if want_lse else None
     if T == 0:
         return (out, lse) if want_lse else out
     lp = lse.data_ptr() if want_lse else 0
@@ -2019,25 +2020,25 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     each = 4 if f32 else 8
     groups = nkv * ((nq // nkv + each - 1) // each)
     keys = _keys_visited(step.max_kv_len, window, page, keep_first, chunk)
-    blocks = 0
+    way = 0
     if f32:
         ns, per = kv4_split_plan_f32(T * groups, keys, sms)
     else:
-        ns, per, blocks = kv4_split_plan(n_seqs, n_seqs * groups, keys, max_pages, sms)
+        ns, per, way = kv4_split_plan(n_seqs, n_seqs * groups, keys, max_pages, sms)
     po = pm = pc = 0
-    if ns > 1:       # (memory of this call's own: two captured graphs, or two streams, share none of it)
+    if ns > 1 and way != 2:      # (memory of this call's own: two captured graphs, or two streams, share none of it)
         n = T * nq * ns
-        part = torch.empty(n * (D + 2) + T * groups, dtype=_F32, device=q.device)
+        part = q.new_empty(n * (D + 2) + T * groups, dtype=_F32)
         po = part.data_ptr()
         pm = po + 4 * n * D
         pc = pm + 8 * n
     args = _KV4_ATTN.pack(qp, p, table, sl, lens, seq, cu, out.data_ptr(), lp, po, pm, pc, err, sk, T, n_seqs, n_slots, nq,
-                          nkv, max_pages, n_pages, window, ns, per, blocks > 0, keep_first, chunk, scale_log2, cap_log2,
+                          nkv, max_pages, n_pages, window, ns, per, way, keep_first, chunk, scale_log2, cap_log2,
                           cap_inv)
     if f32:
         _launch(dev, "attn_kv4_f32", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
     else:
-        _launch(dev, "attn_kv4_decode", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, blocks)
+        _launch(dev, "attn_kv4_decode", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, 4 * sms)
     return (out, lse) if want_lse else out
 
 
@@ -2064,7 +2065,7 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
     w = _take_weights(weights, n_pages, nkv, dev)
     if int(last) < 0:
         raise KernelError("the number of last rows is not negative")
-    blocks = min(65535, max(1, (step.max_kv_len + KV4_PAGE - 1) // KV4_PAGE))
+    blocks = max(1, (step.max_kv_len + 4 * KV4_PAGE - 1) // (4 * KV4_PAGE))       # (a page a warp)
     args = _KV4_WEIGH.pack(qp, lp, p, w, table, sl, lens, cu, T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window,
                            keep_first, chunk, int(last), scale_log2, cap_log2, cap_inv)
     _launch(dev, "kv4_weigh", 1 if T else 0, _fn("attn_kv4", "gb_kv4_weigh", "piip"), args, D, blocks)
@@ -2101,8 +2102,8 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
         if into.shape[0] != n_slots or to_max * KV4_PAGE < min(keep, max_pages * KV4_PAGE):
             raise KernelError(f"the block table of the kept tokens is {tuple(into.shape)} for {keep} tokens of "
                               f"{n_slots} slots")
-    kept = torch.empty((n_seqs, nkv, keep), dtype=_I32, device=pages.device)
-    new = torch.empty((n_seqs,), dtype=_I32, device=pages.device)
+    kept = slots.new_empty((n_seqs, nkv, keep))
+    new = slots.new_empty((n_seqs,))
     if n_seqs == 0:
         return kept, new
     choose = _KV4_CHOOSE.pack(w, table, sl, lens, kept.data_ptr(), new.data_ptr(), n_seqs, n_slots, nkv, max_pages, n_pages,

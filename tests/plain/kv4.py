@@ -23,7 +23,8 @@ def quantise(x):
     lo, hi = g.amin(-1), g.amax(-1)
     m = _down(lo)
     s = -_down(-((hi - m) / torch.full_like(m, 15.0)))
-    c = torch.where(s[..., None] > 0, torch.round((g - m[..., None]) / s[..., None]), torch.zeros_like(g))
+    d = g - m[..., None]                          # rounded to 32 bits; then the nearest code, of two the even one
+    c = torch.where(s[..., None] > 0, torch.round(d.double() / s.double()[..., None]), torch.zeros_like(g, dtype=torch.float64))
     bad = ~(g.isfinite().all(-1) & s.isfinite() & m.isfinite())
     nan = torch.full_like(s, float("nan"))
     c = torch.where(bad[..., None], torch.zeros_like(c), c)

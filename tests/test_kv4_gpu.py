@@ -246,11 +246,12 @@ def test_prompts_in_large_blocks(n):
 
 
 @pytest.mark.parametrize("lens", [[3000, 1, 200, 64, 2500], [33] * 40 + [2000], [700], [2100, 2100, 2100]], ids=lambda x: str(len(x)))
-@pytest.mark.parametrize("least,share", [(None, None), (2, True), (3, True), (9, True), (1, True), (5, False)])
-def test_keys_shared_out_among_the_blocks(lens, least, share, monkeypatch):
-    """Runs of stretches that end inside a pair, hold several pairs, or one pair's middle; padding rows between."""
+@pytest.mark.parametrize("least,way", [(None, None), (2, 1), (3, 1), (9, 1), (1, 1), (5, 0), (15, 2), (40, 2)])
+def test_ways_to_split_the_keys(lens, least, way, monkeypatch):
+    """A block a split; clusters of them; runs of stretches that end inside a pair, hold several pairs, or one pair's
+    middle; padding rows between."""
     monkeypatch.setattr(ops, "KV4_SPLIT_OVERRIDE", least)
-    monkeypatch.setattr(ops, "KV4_SHARE_OVERRIDE", share)
+    monkeypatch.setattr(ops, "KV4_SHARE_OVERRIDE", way)
     c = Cache(lens, 2, 64, seed=len(lens))
     attend(c, [1] * len(lens), 12, torch.bfloat16, sinks=True, pad=2)
     attend(c, [1] * len(lens), 4, torch.bfloat16, window=300, keep_first=40)
