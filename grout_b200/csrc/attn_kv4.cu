@@ -126,7 +126,7 @@ __device__ __forceinline__ void empty_row(const Kv4AttnArgs& a, int seq, int gro
 template <int D>
 struct Kv4Decode {
   static constexpr int WARPS = 4;
-  static constexpr int STAGES = 2;
+  static constexpr int STAGES = 2;                              // (two: the code that gives up knows)
   static constexpr int UNIT = 32;                               // keys of a stage: whole records of one page
   static constexpr int RECORDS = UNIT / KV4_TOKENS;
   static constexpr int STAGE_BYTES = RECORDS * Kv4<D>::RECORD;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
   const int keep = a.window > 0 ? a.keep_first : 0;
   uint8_t* ring = smem + warp * C::STAGES * C::STAGE_BYTES;
   const uint32_t magic = kv4_magic(a.n_seqs);
-  uint32_t parity = 0;                               // the phases to wait for, by stage
+  uint32_t turn = 0;                                 // stretches that this warp has taken: its stage and its phase follow
   bool ok = true;
 
   // this block's run [at, end) of the list of all stretches; before[i]: those of one pair of each sequence in front of i
@@ -359,36 +359,36 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
   }
   if (!more) return;
 
-  // The part that is worked on: its sequence's last position and first key, its stretches [v, v_end) of this warp, what
-  // is on its way.  begin() finds the block's next part and asks for its first stretches; the results of the part
-  // before are put together while they come.
-  int pos = 0, lo = 0, v = 0, v_end = 0, gap_at = 0, gap = 0, page_next = 0;
+  // The part that is worked on: its sequence's last position and first key, this warp's `mine` stretches from v on (every
+  // fourth of the block's).  begin() finds the block's next part and asks for its first stretches; the results of the
+  // part before are put together while they come.
+  int pos = 0, lo = 0, v = 0, mine = 0, gap_at = 0, gap = 0;
   const int* table = nullptr;
   const uint8_t* head = nullptr;                     // the kv head's records of page 0
-  uint32_t asked = 0;                                // stages with something on its way
   bool lost = false;                                 // a page that there is not: the result is NaN
+  int pages = 0;                                     // lane i: the page of the i-th of 32 stretches
   const size_t page_bytes = (size_t)a.nkv * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
   auto first_of = [&](int u) { return (BOUNDED && u >= gap_at ? u + gap : u) * C::UNIT; };
-  // The page of a stretch is looked up a turn before the stretch is asked for: the answer takes hundreds of cycles, in
-  // which a warp that needs it does nothing else.
-  auto page_of = [&](int u) {
-    return u < v_end ? kv4_page(table, first_of(u) / KV4_PAGE, a.max_pages, a.n_pages) : 0;
-  };
-  // asks for stretch u (a whole warp calls; one lane asks): true when something comes
-  auto ask = [&](int u, int page, int stage) {
-    if (page < 0) {
-      lost = true;
-      return false;
+  // looks up the pages of stretches k .. k + 31 of this warp's
+  auto look_up = [&](int k) {
+    pages = 0;
+    if (k + lane < mine) {
+      pages = kv4_page(table, first_of(v + (k + lane) * C::WARPS) / KV4_PAGE, a.max_pages, a.n_pages);
+      lost = lost || pages < 0;
+      pages = max(pages, 0);
     }
+  };
+  // asks for stretch k of this warp's (the whole warp calls; one lane asks)
+  auto ask = [&](int k, uint32_t at_turn) {
+    const int page = __shfl_sync(0xffffffffu, pages, k & 31), key0 = first_of(v + k * C::WARPS);
+    const uint32_t stage = at_turn % C::STAGES;
     if (elect_one()) {
-      const int key0 = first_of(u);
       const uint32_t bytes = min(NR, (pos - key0) / KV4_TOKENS + 1) * F::RECORD;
       mbar_expect_tx(&full[warp][stage], bytes);
       bulk_load(ring + stage * C::STAGE_BYTES, head + page * page_bytes + key0 % KV4_PAGE / KV4_TOKENS * F::RECORD, bytes,
                 &full[warp][stage]);
     }
     __syncwarp();
-    return true;
   };
   int turn_of = 0;                                   // which of part_s has the part that is worked on
   auto begin = [&]() {
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     const bool live = find_row(a, part.seq, pos);
     const int slot = live ? a.slots[part.seq] : 0;
     const Stretches list(pos, C::UNIT, BOUNDED ? a.window : 0, BOUNDED ? a.keep_first : 0, BOUNDED ? a.chunk : 0);
-    int v_begin;
+    int v_begin, v_end;
     if (a.shared == 1) {
       const unsigned first = (unsigned)before[part.seq] * groups, n = (unsigned)list.n;
       part.group = (int)((at - first) / n);
@@ -419,18 +419,15 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     }
     if (threadIdx.x == 0) part_s[turn_of] = part;
     v = v_begin + warp;
+    mine = ok ? max(0, (v_end - v + C::WARPS - 1) / C::WARPS) : 0;
     lo = list.lo, gap_at = list.n_kept, gap = list.first - list.n_kept;
     table = a.block_table + (size_t)slot * a.max_pages;
     head = a.pages + (size_t)(part.group / hgroups) * (KV4_PAGE / KV4_TOKENS) * F::RECORD;
     lost = a.n_splits > 1 && part.n_pieces > a.n_splits;   // (keys beyond the caller's bound of the lengths)
-    asked = 0;
-    int page[C::STAGES + 1];
+    look_up(0);
 #pragma unroll
-    for (int s = 0; s <= C::STAGES; ++s) page[s] = page_of(v + s * C::WARPS);
-#pragma unroll
-    for (int s = 0; s < C::STAGES; ++s)
-      if (ok && v + s * C::WARPS < v_end && ask(v + s * C::WARPS, page[s], s)) asked |= 1u << s;
-    page_next = page[C::STAGES];
+    for (int k = 0; k < C::STAGES; ++k)
+      if (k < mine) ask(k, turn + k);
     return part;
   };
 
@@ -470,16 +467,19 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
         for (int c = 0; c < 4; ++c) o[g][i][c] = 0.f;
     }
 
-    int stage = 0;
 #pragma unroll 1
-    for (; v < v_end && ok; v += C::WARPS) {
-      const int page_now = page_next;
-      page_next = page_of(v + (C::STAGES + 1) * C::WARPS);
-      if (asked >> stage & 1) {
-        if (!mbar_wait_warp(&full[warp][stage], parity >> stage & 1, nullptr)) { ok = false; break; }
-        parity ^= 1u << stage;
+    for (int k = 0; k < mine; ++k, ++turn) {
+      {
+        const uint32_t stage = turn % C::STAGES;
+        if (!mbar_wait_warp(&full[warp][stage], turn / C::STAGES & 1, nullptr)) {
+          // gave up: wait for what is still on its way, say so, go on to the block's barriers (the result is void)
+          if (k + 1 < mine) mbar_wait_warp(&full[warp][(turn + 1) % C::STAGES], (turn + 1) / C::STAGES & 1, nullptr);
+          if (lane == 0) atomicCAS(a.error, 0, GB_ERR_KV4_TIMEOUT);
+          ok = false;
+          break;
+        }
         const uint8_t* unit = ring + stage * C::STAGE_BYTES;
-        const int key0 = first_of(v);
+        const int key0 = first_of(v + k * C::WARPS);
         float s[NR][4];
         uint32_t vp[NR][2][NG];                      // the values' pairs of this lane's two rows
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
             down = __uint_as_float((uint32_t)(254 - e) << 23);
             s_most = __uint_as_float((uint32_t)(e + 6) << 23);
           }
-          const float turn = down / s_down;
+          const float change = down / s_down;
           s_down = down;
           x0 = fmaxf(x0, m[0]), x1 = fmaxf(x1, m[1]);
           const float f0 = m[0] == -INFINITY ? 0.f : exp2_fast(m[0] - x0);
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[g][i][c] *= ((c & 1) ? f1 : f0) * turn;
+              for (int c = 0; c < 4; ++c) o[g][i][c] *= ((c & 1) ? f1 : f0) * change;
           }
         }
 #pragma unroll
@@ -587,19 +587,15 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
             for (int i = 0; i < 4; ++i) mma_f16(o[g][i], ya[i], za[i], yb[i], zb[i], p0, p1);
           }
         }
-        asked &= ~(1u << stage);
         __syncwarp();                                  // all lanes have read the stage
       }
-      const int next = v + C::STAGES * C::WARPS;
-      if (next < v_end && ask(next, page_now, stage)) asked |= 1u << stage;
-      stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+      const int next = k + C::STAGES;
+      if (next < mine) {
+        if ((next & 31) == 0) look_up(next);
+        ask(next, turn + C::STAGES);
+      }
     }
-    if (!ok && asked) {                                // gave up: wait for what is still on its way, say so, go on to
-      for (int s = 0; s < C::STAGES; ++s)              // the block's barriers (the result is void)
-        if (asked >> s & 1) mbar_wait_warp(&full[warp][s], parity >> s & 1, nullptr);
-      if (lane == 0) atomicCAS(a.error, 0, GB_ERR_KV4_TIMEOUT);
-    }
-    if (lost) m[0] = m[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
+    if (__any_sync(0xffffffffu, lost)) m[0] = m[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
 
     const bool again = more;
     turn_of ^= 1;
