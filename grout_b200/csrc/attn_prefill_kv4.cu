@@ -21,6 +21,23 @@ struct Kv4Pages {
   __device__ __forceinline__ static int slot(const Params& p, int s) { return s < p.n_slots ? s : -1; }
   __device__ __forceinline__ static void before_padding() { pdl_wait(); }
   __device__ __forceinline__ static void prepare(const Params&) {}
+  // C tanh(x) log2 e = C log2 e (1 - 2 / (2^(2 x log2 e) + 1)) with the special unit's power and inverse as they are
+  // (2^-22 of their size off; no power is 0 and an infinite one's inverse is 0, which are the two ends) and two scores
+  // to an instruction around them.  CAP_US
+  __device__ __forceinline__ static void cap_scores(float (&s)[AT_BN], const ScoreCap& cap) {
+    const float in = cap.cap_inv * 2.8853900817779268f;
+    const uint64_t in2 = pack_f32x2(in, in), zero2 = pack_f32x2(0.f, 0.f), one2 = pack_f32x2(1.f, 1.f);
+    const uint64_t twice2 = pack_f32x2(-2.f * cap.cap_log2, -2.f * cap.cap_log2), top2 = pack_f32x2(cap.cap_log2, cap.cap_log2);
+#pragma unroll
+    for (int c = 0; c < AT_BN; c += 2) {
+      float x0, x1, r0, r1;
+      unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), in2, zero2), x0, x1);
+      unpack_f32x2(add_f32x2(pack_f32x2(fast_exp2(x0), fast_exp2(x1)), one2), x0, x1);
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(x0));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(x1));
+      unpack_f32x2(fma_f32x2(pack_f32x2(r0, r1), twice2, top2), s[c], s[c + 1]);
+    }
+  }
 
   // What a lane needs of a half row of a key and of a value, and whether its token is one that the block sees.
   template <int D>
@@ -57,16 +74,20 @@ struct Kv4Pages {
     }
   }
 
-  // 1 + c / 16 in both halves -> s c + m (s16: 16 s): c / 16 is exact, the multiply-add rounds once.
-  static __device__ __forceinline__ uint32_t element2(uint32_t x, __nv_bfloat162 s16, __nv_bfloat162 m) {
-    const __nv_bfloat162 one = __floats2bfloat162_rn(1.f, 1.f);
-    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), one);
-    const __nv_bfloat162 y = __hfma2(s16, c, m);
+  // The eight elements of a word, s c + m: a code in the low bits of 128's mantissa is 128 + c, less 128 it is c, exactly,
+  // and the multiply-add rounds once.  `magic` is 128 in both halves, from a register: with two constants an instruction
+  // the compiler makes two of it.
+  template <int I>
+  static __device__ __forceinline__ uint32_t element2(uint32_t w, uint32_t magic, __nv_bfloat162 s, __nv_bfloat162 m) {
+    uint32_t x;                                            // (w >> 4 I & 0x000f000f) | magic
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> (4 * I)), "n"(0x000f000fu), "r"(magic));
+    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(128.f, 128.f));
+    const __nv_bfloat162 y = __hfma2(s, c, m);
     return *reinterpret_cast<const uint32_t*>(&y);
   }
-  static __device__ __forceinline__ void unpack8(uint32_t addr, uint32_t w, __nv_bfloat162 s16, __nv_bfloat162 m) {
-    sts128(addr, element2(kv4_two<0>(w), s16, m), element2(kv4_two<1>(w), s16, m), element2(kv4_two<2>(w), s16, m),
-           element2(kv4_two<3>(w), s16, m));
+  static __device__ __forceinline__ void unpack8(uint32_t addr, uint32_t w, uint32_t magic, __nv_bfloat162 s, __nv_bfloat162 m) {
+    sts128(addr, element2<0>(w, magic, s, m), element2<1>(w, magic, s, m), element2<2>(w, magic, s, m),
+           element2<3>(w, magic, s, m));
   }
 
   template <int DS, int G>
@@ -76,6 +97,7 @@ struct Kv4Pages {
     constexpr int EACH = 2 * AT_BN / (32 * Cfg::PRODUCERS);          // half rows of a lane
     using F = Kv4<D>;
     const int lane = threadIdx.x & 31;
+    const uint32_t magic = 0x43004300u ^ (uint32_t)(a.n_seqs >> 31);
     Half<D> next[EACH];
     auto ask = [&](int j) {
       const int tile = b.tile(j);
@@ -136,7 +158,7 @@ struct Kv4Pages {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           if (poison) kp[g] = 0x7fff7fffu, vp[g] = 0u;
-          const float s1 = 16.f * kv4_s(kp[g]), m1 = kv4_m(kp[g]), s2 = 16.f * kv4_s(vp[g]), m2 = kv4_m(vp[g]);
+          const float s1 = kv4_s(kp[g]), m1 = kv4_m(kp[g]), s2 = kv4_s(vp[g]), m2 = kv4_m(vp[g]);
           ks[g] = __floats2bfloat162_rn(s1, s1), km[g] = __floats2bfloat162_rn(m1, m1);
           vs[g] = __floats2bfloat162_rn(s2, s2), vm[g] = __floats2bfloat162_rn(m2, m2);
         }
@@ -149,12 +171,12 @@ struct Kv4Pages {
           const int w = (i % W) ^ half, t = 2 * half + i / W;
           const int g = w / 2, chunk = (w & 1) * 4 + t;
           const uint32_t word = half ? now[u].k[i ^ 1] : now[u].k[i];
-          unpack8(krow + g * Cfg::SUB_BYTES + ((uint32_t)(chunk ^ swz) << 4), real ? word : 0u, ks[(i % W) / 2], km[(i % W) / 2]);
+          unpack8(krow + g * Cfg::SUB_BYTES + ((uint32_t)(chunk ^ swz) << 4), real ? word : 0u, magic, ks[(i % W) / 2], km[(i % W) / 2]);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           const int g = i % NG, chunk = (4 * half + i / NG) ^ F::turn(row);
-          unpack8(vrow + g * Cfg::SUB_BYTES + ((uint32_t)(chunk ^ swz) << 4), real && !poison ? now[u].v[i] : 0u, vs[g], vm[g]);
+          unpack8(vrow + g * Cfg::SUB_BYTES + ((uint32_t)(chunk ^ swz) << 4), real && !poison ? now[u].v[i] : 0u, magic, vs[g], vm[g]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // visible to the tensor core

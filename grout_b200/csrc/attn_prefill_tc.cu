@@ -11,6 +11,10 @@ struct TmaPages {
   __device__ __forceinline__ static constexpr float* lse(const Params&) { return nullptr; }
   __device__ __forceinline__ static int slot(const Params&, int s) { return s; }
   __device__ __forceinline__ static void before_padding() {}
+  __device__ __forceinline__ static void cap_scores(float (&s)[AT_BN], const ScoreCap& cap) {
+#pragma unroll
+    for (int c = 0; c < AT_BN; ++c) s[c] = capped_log2(s[c] * cap.cap_inv, cap);
+  }
   __device__ __forceinline__ static void prepare(const Params& p) {
     tma_prefetch_map(&p.k);
     tma_prefetch_map(&p.v);

@@ -519,10 +519,7 @@ attn_prefill_tc_kernel(const __grid_constant__ typename Source::Params source, c
         __syncwarp();
         mbar_arrive_if(&s_empty[g], lane == 0);   // S is in registers: the next S may be written
         AT_STAMP(stamp_buf, (g * 4 + (j - 8)) * 8 + 2)
-        if (capped) {   // scores enter the log2 domain here, through the cap
-#pragma unroll
-          for (int c = 0; c < AT_BN; ++c) s[c] = capped_log2(s[c] * a.cap.cap_inv, a.cap);
-        }
+        if (capped) Source::cap_scores(s, a.cap);   // scores enter the log2 domain here, through the cap
         if (need_mask) {
           const int last = hi - key0, first = lo - key0;   // this row's keys of the tile
           if (bounded) {

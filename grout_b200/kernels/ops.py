@@ -1910,6 +1910,7 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
     return out
 
 
+KV4_PER_SM = 4             # blocks of the bfloat16 kernel that an SM holds
 KV4_LEAST = 8              # stretches of 32 keys that a block takes at least (two for each of its warps)
 KV4_SPLIT_OVERRIDE: Optional[int] = None      # stretches that a block takes at least, for experiments
 KV4_SHARE_OVERRIDE: Optional[int] = None      # how pairs are split (0, 1 or 2, see kv4_split_plan), for tests
@@ -1922,7 +1923,7 @@ def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int)
     stretches out, at least so many each, and a pair has at most so many splits."""
     tiles = max(1, (keys + 31) // 32)
     least = KV4_SPLIT_OVERRIDE or max(KV4_LEAST, -(-tiles // 62))
-    splits, blocks, way = -(-tiles // least), 4 * sms, KV4_SHARE_OVERRIDE
+    splits, blocks, way = -(-tiles // least), KV4_PER_SM * sms, KV4_SHARE_OVERRIDE
     if splits == 1:
         return 1, tiles, 0
     if way is None:
@@ -2038,7 +2039,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     if f32:
         _launch(dev, "attn_kv4_f32", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
     else:
-        _launch(dev, "attn_kv4_decode", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, 4 * sms)
+        _launch(dev, "attn_kv4_decode", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, KV4_PER_SM * sms)
     return (out, lse) if want_lse else out
 
 
