@@ -927,23 +927,25 @@ struct Kv4WeighArgs {
 };
 
 #define WEIGH_WARPS 4
+#define WEIGH_RECORDS 2      // of a step
 
 // weights[j] += the sum over the sequence's last rows and the kv head's query heads of 2^(s_j c - lse).  The (row, head)
-// pairs are the columns of the products, eight at a time; a warp has a page of 64 tokens of one kv head, whose keys it
-// asks for all at once, and adds the sums of one set of columns after the other to its tokens' weights: nobody else
-// touches them, and the order is always the same.
+// pairs are the columns of the products, eight at a time.  A warp takes 32 tokens of one kv head at a time, every
+// (WEIGH_WARPS x blocks)th of them, with the keys of the next on their way while it sums this one's; nobody else touches
+// these tokens' weights, and the order of the sums is always the same.  More than eight columns: a set after the other,
+// the keys read again for each (they come from L2).
 template <int D>
-__global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4WeighArgs a) {
+__global__ void __launch_bounds__(WEIGH_WARPS * 32, 4) kv4_weigh_kernel(const Kv4WeighArgs a) {
   using F = Kv4<D>;
-  constexpr int NG = F::NG, NR = KV4_PAGE / KV4_TOKENS;
+  constexpr int NG = F::NG, NR = WEIGH_RECORDS, STEP = NR * KV4_TOKENS;
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, seq = blockIdx.z, G = a.nq / a.nkv;
   const int slot = a.slots[seq], len = a.kv_len[seq];
   const int row1 = a.cu_q[seq + 1], row_first = a.cu_q[seq];
-  const int n_pages = (int)min((len + (long long)KV4_PAGE - 1) / KV4_PAGE, (long long)a.max_pages);
-  int tile = blockIdx.x * WEIGH_WARPS + warp;
-  if ((unsigned)slot >= (unsigned)a.n_slots || tile >= n_pages) return;
+  const int steps = (int)min((len + (long long)STEP - 1) / STEP, (long long)a.max_pages * (KV4_PAGE / STEP));
+  const int stride = gridDim.x * WEIGH_WARPS, step0 = blockIdx.x * WEIGH_WARPS + warp;
+  if ((unsigned)slot >= (unsigned)a.n_slots || step0 >= steps) return;
   const int row0 = a.last > 0 ? max(row_first, row1 - a.last) : row_first;
   if (row0 >= row1 || row_first < 0 || row1 > a.n_rows) return;
   const int pos0 = len - (row1 - row0);                          // the position of row0
@@ -952,73 +954,90 @@ __global__ void __launch_bounds__(WEIGH_WARPS * 32) kv4_weigh_kernel(const Kv4We
   const int keep = a.window > 0 ? a.keep_first : 0;
   const uint32_t magic = kv4_magic(a.n_seqs);
   const int tok = kv4_token(r), columns = (row1 - row0) * G;
-  const bool capped = a.cap.cap_log2 != 0.f;
-  // column c is head c % G of row c / G; this lane loads the query of column r of a set and sums columns 2 t, 2 t + 1
-  auto query = [&](int c) {
-    return c < columns ? a.q + ((size_t)(row0 + c / G) * a.nq + kvh * G + c % G) * D : nullptr;
+  const bool capped = a.cap.cap_log2 != 0.f, bounded = a.window > 0 || a.chunk > 0;
+
+  uint32_t ka[NR][D / 32], kb[NR][D / 32], pa[NR][NG], pb[NR][NG];
+  // the record of the head that step s begins with, or null: nothing to do there
+  auto record_of = [&](int s) -> const uint8_t* {
+    if (s >= steps || (s * STEP + STEP <= lowest && s * STEP >= keep)) return nullptr;
+    const int page = kv4_page(table, s * STEP / KV4_PAGE, a.max_pages, a.n_pages);
+    if (page < 0) return nullptr;
+    return a.pages + (((size_t)page * a.nkv + kvh) * (KV4_PAGE / KV4_TOKENS) + s * STEP % KV4_PAGE / KV4_TOKENS) * F::RECORD;
   };
-  Kv4Query<D> q;
-  q.load(query(r));
-  for (; tile < n_pages; tile += gridDim.x * WEIGH_WARPS) {
-    const int key0 = tile * KV4_PAGE;
-    if (key0 + KV4_PAGE <= lowest && key0 >= keep) continue;
-    const int page = kv4_page(table, tile, a.max_pages, a.n_pages);
-    if (page < 0) continue;
-    const size_t at = (size_t)page * a.nkv + kvh;
-    uint32_t ka[NR][D / 32], kb[NR][D / 32], pa[NR][NG], pb[NR][NG];
+  auto load = [&](const uint8_t* b) {
+    if (!b) return;
 #pragma unroll
-    for (int u = 0; u < NR; ++u) {
-      const uint8_t* b = a.pages + (at * NR + u) * F::RECORD;
+    for (int u = 0; u < NR; ++u, b += F::RECORD) {
       load_words(b + tok * F::ROW + t * (D / 8), ka[u]);
       load_words(b + (tok + 8) * F::ROW + t * (D / 8), kb[u]);
       load_words(b + F::PAIR_OFF + tok * F::PAIR, pa[u]);
       load_words(b + F::PAIR_OFF + (tok + 8) * F::PAIR, pb[u]);
     }
-    float* w = a.weights + at * KV4_PAGE;
-    float sum[NR][2];
+  };
+  for (int c0 = 0; c0 < columns; c0 += 8) {
+    const uint8_t* here = record_of(step0);
+    load(here);
+    const uint8_t* after = record_of(step0 + stride);
+    // column c is head c % G of row c / G; this lane loads the query of column c0 + r and sums columns c0 + 2 t, + 2 t + 1
+    Kv4Query<D> q;
+    {
+      const int c = c0 + r;
+      q.load(c < columns ? a.q + ((size_t)(row0 + c / G) * a.nq + kvh * G + c % G) * D : nullptr);
+    }
+    int last[2], first[2];
+    float lse[2], factor[2];
 #pragma unroll
-    for (int u = 0; u < NR; ++u) sum[u][0] = sum[u][1] = 0.f;
-    for (int c0 = 0; c0 < columns; c0 += 8) {
-      if (columns > 8) q.load(query(c0 + r));
-      // what this lane's two columns see, and their factors
-      int last[2], first[2];
-      float lse[2], factor[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = c0 + 2 * t + i, row = row0 + c / G;
-        last[i] = -1, first[i] = 0, lse[i] = 0.f;
-        if (c < columns) {
-          lse[i] = a.lse[(size_t)row * a.nq + kvh * G + c % G] * 1.4426950408889634f;
-          if (lse[i] != -INFINITY) last[i] = pos0 + row - row0, first[i] = first_key(max(last[i], 0), a.window, a.chunk);
-        }
-        factor[i] = (capped ? a.cap.cap_inv : a.scale_log2) * q.back[i];
+    for (int i = 0; i < 2; ++i) {
+      const int c = c0 + 2 * t + i, row = row0 + c / G;
+      last[i] = -1, first[i] = 0, lse[i] = 0.f;
+      if (c < columns) {
+        lse[i] = a.lse[(size_t)row * a.nq + kvh * G + c % G] * 1.4426950408889634f;
+        if (lse[i] != -INFINITY) last[i] = pos0 + row - row0, first[i] = first_key(max(last[i], 0), a.window, a.chunk);
       }
+      factor[i] = (capped ? a.cap.cap_inv : a.scale_log2) * q.back[i];
+    }
+    for (int s = step0; s < steps; s += stride) {
+      float sum[NR][2];
 #pragma unroll
       for (int u = 0; u < NR; ++u) {
-        float s[4];
-        kv4_scores<D>(ka[u], kb[u], pa[u], pb[u], q, magic, s);
+        float x[4];
+        if (here) kv4_scores<D>(ka[u], kb[u], pa[u], pb[u], q, magic, x);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int half = 0; half < 2; ++half) {
+          const int j = s * STEP + u * KV4_TOKENS + tok + half * 8;
+          sum[u][half] = 0.f;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int j = key0 + u * KV4_TOKENS + tok + half * 8;
-            float x = s[2 * half + i] * factor[i];
-            if (capped) x = capped_log2(x, a.cap);
-            const float p = exp2_fast(x - lse[i]);
-            if (j <= last[i] && (j >= first[i] || j < keep)) sum[u][half] += p;
+          for (int i = 0; i < 2; ++i) {
+            float y = x[2 * half + i] * factor[i];
+            if (capped) y = capped_log2(y, a.cap);
+            const float p = exp2_fast(y - lse[i]);
+            if (j <= last[i] && (!bounded || j >= first[i] || j < keep)) sum[u][half] += p;
           }
+        }
       }
+      const bool done = here != nullptr;
+      const int page_at = s * STEP;
+      float* w = a.weights;
+      if (done) {
+        const int page = kv4_page(table, page_at / KV4_PAGE, a.max_pages, a.n_pages);
+        w += ((size_t)page * a.nkv + kvh) * KV4_PAGE + page_at % KV4_PAGE;
+      }
+      here = after;
+      load(here);
+      after = record_of(s + 2 * stride);
+      if (!done) continue;
+#pragma unroll
+      for (int u = 0; u < NR; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 1);
+          sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 2);
+          // Each lane of a row's four has one of its tokens of the step.  (Added where it lies, without waiting for what
+          // is there; this lane alone adds to it, in the order of the sets, so the sum is the same every time.)
+          const int j = u * KV4_TOKENS + tok + half * 8;
+          if (t == u * 2 + half && page_at + j < len) atomicAdd(w + j, sum[u][half]);
+        }
     }
-#pragma unroll
-    for (int u = 0; u < NR; ++u)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 1);
-        sum[u][half] += __shfl_xor_sync(0xffffffffu, sum[u][half], 2);
-        // (a lane of each row's four has a record's two tokens)
-        const int j = u * KV4_TOKENS + tok + half * 8;
-        if (t == u && key0 + j < len) w[j] += sum[u][half];
-      }
   }
 }
 
