@@ -59,6 +59,7 @@ class SequenceCache:
         self.max_slots = min(max_slots, n_pages)
         self.slots = SlotList(self.max_slots)
         self.length: Dict[int, int] = {}
+        self.dropped: Dict[int, int] = {}    # tokens let go of: the next one's position is its place plus these
         self.stores: List[Any] = []
         self.sizes = StoreSizes(n_pages=n_pages, max_slots=self.max_slots,
                                 max_pages_per_seq=min(pages_for(max_seq_len), n_pages),
@@ -74,7 +75,7 @@ class SequenceCache:
         slot = self.slots.acquire()
         for st in self.stores:
             st.open(slot)
-        self.length[slot] = 0
+        self.length[slot] = self.dropped[slot] = 0
         return slot
 
     def reserve(self, slot: int, new_tokens: int) -> None:
@@ -91,11 +92,33 @@ class SequenceCache:
         for st in self.stores:
             st.trim(slot, self.length[slot])
 
+    def evict(self, slots: Sequence[int], keep: int, recent: int, first: int = 0) -> None:
+        """Cuts the sequences in ``slots`` that hold more than ``keep`` tokens to ``keep``: every kv head of every layer
+        keeps their ``first`` tokens, their ``recent`` newest, and of the others those that were paid the most attention.
+        The next token of such a sequence keeps its position (``dropped`` tells it from its place).  Refused, before
+        anything is changed, unless all stores of keys and values are in 4 bits, keep weights and are whole."""
+        keep, recent, first = int(keep), int(recent), int(first)
+        if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
+            raise ValueError(f"{first} first and {recent} recent tokens do not fit {keep} that are kept")
+        slots = [s for s in dict.fromkeys(slots) if self._len(s) > keep]
+        for st in self.stores:
+            if not callable(getattr(st, "check_evict", None)):
+                raise ValueError(f"a store for {getattr(st, 'spec', st)!r} does not let go of tokens")
+            st.check_evict()
+        if not slots:
+            return
+        lengths = [self.length[s] for s in slots]
+        for st in self.stores:
+            st.evict(slots, lengths, keep, recent, first)
+        for s, n in zip(slots, lengths):
+            self.length[s] = keep
+            self.dropped[s] += n - keep
+
     def close(self, slot: int) -> None:
         self._len(slot)
         for st in self.stores:
             st.close(slot)
-        del self.length[slot]
+        del self.length[slot], self.dropped[slot]
         self.slots.release(slot)
 
     def _len(self, slot: int) -> int:

@@ -38,16 +38,23 @@ class KVSpec:
     with a window, a sequence's first ``keep_first`` tokens stay visible to every
     later query, so the pages that hold them are never given back.  ``chunk``: queries see
     the tokens of their own chunk of that many positions only (positions count from the
-    sequence's start), so what lies in front of the next token's chunk is given back."""
+    sequence's start), so what lies in front of the next token's chunk is given back.  ``bits`` 4: the
+    store holds 4-bit codes (None: the engine's type), and with ``weighed`` beside every token the
+    attention that it has been paid, by which ``SequenceCache.evict`` lets go of tokens."""
     n_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     values_in_keys: bool = False
     keep_first: int = 0
     chunk: Optional[int] = None
+    bits: Optional[int] = None
+    weighed: bool = False
 
     def make_store(self, n_layers: int, sizes: StoreSizes, dtype, device, allocate: bool = True):
-        from .stores import KVStore
+        from .stores import KVStore, Kv4Store
+        if self.bits is not None:
+            return Kv4Store(self, n_layers, sizes.n_pages, sizes.max_slots, sizes.max_pages_per_seq,
+                            device, allocate)
         return KVStore(self, n_layers, sizes.n_pages, sizes.max_slots, sizes.max_pages_per_seq,
                        dtype, device, allocate)
 

@@ -9,6 +9,9 @@ zero-filled once and never cleared again: a sequence's length gates every read. 
 src/model.rs:1450-1455.)  A store with a window (or chunks) gives pages back as soon
 as every token in them has left the window (the chunk) of all later queries.
 
+``Kv4Store``: the same pages with keys and values in 4 bits, ``[layers, pages, kv heads, 4, record]`` of bytes, and the
+tokens' weights ``[layers, pages, kv heads, PAGE_TOKENS]`` where they are kept.
+
 ``StateStore``: ``[layers, slots + 1, *shape]`` of fixed-size state, zeroed when a
 slot is opened; the last row belongs to no sequence and is where padding rows
 (slot -1) may be pointed, so that a mixer needs no branch for them (the reference's packed backend keeps such state per layer,
@@ -35,6 +38,16 @@ class KVLayerView:
     """What an attention layer sees of its store."""
     k_pages: torch.Tensor        # [pages, kv heads, PAGE_TOKENS, head_dim]
     v_pages: torch.Tensor
+    block_table: torch.Tensor    # int32 [slots, pages per sequence]
+    page: int
+    spec: KVSpec
+
+
+@dataclass
+class Kv4LayerView:
+    """What an attention layer sees of a store in 4 bits."""
+    pages: torch.Tensor          # uint8 [pages, kv heads, 4, record]
+    weights: Optional[torch.Tensor]     # float32 [pages, kv heads, PAGE_TOKENS]
     block_table: torch.Tensor    # int32 [slots, pages per sequence]
     page: int
     spec: KVSpec
@@ -104,6 +117,9 @@ class KVStore:
                 self.pool.release(pages[i])
                 pages[i] = None
 
+    def check_evict(self) -> None:
+        raise ValueError("tokens are let go of by weight from a cache in 4 bits that keeps weights only")
+
     def close(self, slot: int) -> None:
         for p in self.pages_of.pop(slot):
             if p is not None:
@@ -137,6 +153,47 @@ class KVStore:
             raise AssertionError("held pages and the sequences' pages differ")
 
 
+class Kv4Store(KVStore):
+    """Keys and values in 4 bits."""
+
+    def __init__(self, spec: KVSpec, n_layers: int, n_pages: int, max_slots: int, max_pages_per_seq: int,
+                 device, allocate: bool = True):
+        if spec.bits != 4 or spec.head_dim not in (64, 128) or spec.values_in_keys:
+            raise ValueError(f"no cache for {spec}: 4 bits, heads of 64 or 128, keys and values of their own")
+        super().__init__(spec, n_layers, n_pages, max_slots, max_pages_per_seq, torch.uint8, device, allocate=False)
+        self.pages = self.weights = None
+        if allocate:
+            rows = (n_layers, max(n_pages, 1), spec.n_kv_heads)
+            self.pages = torch.zeros(rows + (4, 18 * spec.head_dim), dtype=torch.uint8, device=self.device)
+            if spec.weighed:
+                self.weights = torch.zeros(rows + (PAGE_TOKENS,), dtype=torch.float32, device=self.device)
+            self.table_dev = torch.zeros((max_slots, max_pages_per_seq), dtype=torch.int32, device=self.device)
+
+    def layer(self, index: int) -> Kv4LayerView:
+        return Kv4LayerView(self.pages[index], None if self.weights is None else self.weights[index], self.table_dev,
+                            PAGE_TOKENS, self.spec)
+
+    def check_evict(self) -> None:
+        if not self.spec.weighed or self.spec.window is not None or self.spec.chunk is not None:
+            raise ValueError("tokens are let go of by weight from a cache that keeps weights and has neither a window "
+                             f"nor chunks, not from {self.spec}")
+
+    def evict(self, slots: List[int], lengths: List[int], keep: int, recent: int, first: int) -> None:
+        """Cuts sequences of more than ``keep`` tokens to ``keep`` in every layer (``ops.kv4_evict``) and gives the
+        pages behind them back."""
+        if self.pages is not None:
+            from ..kernels import ops
+            self.flush()
+            where, lens = (torch.tensor(x, dtype=torch.int32, device=self.device) for x in (slots, lengths))
+            for pages, weights in zip(self.pages, self.weights):
+                ops.kv4_evict(pages, weights, self.table_dev, slots=where, kv_len=lens, page=PAGE_TOKENS, keep=keep,
+                              recent=recent, first=first)
+        for slot in slots:
+            pages = self.pages_of[slot]
+            self.pool.release_many(pages[pages_for(keep):])
+            del pages[pages_for(keep):]
+
+
 class StateStore:
     def __init__(self, spec: StateSpec, n_layers: int, max_slots: int, device, allocate: bool = True):
         self.spec, self.n_layers, self.max_slots = spec, n_layers, max_slots
@@ -159,6 +216,12 @@ class StateStore:
 
     def trim(self, slot: int, length: int) -> None:
         pass
+
+    def check_evict(self) -> None:
+        pass
+
+    def evict(self, slots, lengths, keep, recent, first) -> None:
+        pass                     # (a state has no tokens to let go of)
 
     def close(self, slot: int) -> None:
         self.open_slots.remove(slot)
@@ -194,6 +257,14 @@ class SideBySideStore:
     def trim(self, slot: int, length: int) -> None:
         for st in self.stores:
             st.trim(slot, length)
+
+    def check_evict(self) -> None:
+        for st in self.stores:
+            st.check_evict()
+
+    def evict(self, slots, lengths, keep, recent, first) -> None:
+        for st in self.stores:
+            st.evict(slots, lengths, keep, recent, first)
 
     def close(self, slot: int) -> None:
         for st in self.stores:

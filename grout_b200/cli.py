@@ -67,6 +67,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--quiet", action="store_true",
                     help="do not print the generated text or the profile, only the times")
     ap.add_argument("--fp32", action="store_true", help="run the true 32-bit path")
+    ap.add_argument("--cache-bits", type=int, choices=[4], default=None,
+                    help="keep keys and values in 4 bits (attention with heads of 64 or 128)")
     ap.add_argument("--output-json", default=None, help="write token ids, counts and seconds here")
     ap.add_argument("--device", default="cuda:0")
     return ap
@@ -106,10 +108,10 @@ def main(argv: Optional[List[str]] = None) -> int:
     if random_config is not None:
         with open(random_config, encoding="utf-8") as fh:
             engine = Engine.random(json.load(fh), args.seed, dtype=dtype, device=args.device,
-                                   max_seq_len=args.max_seq_len, max_batch=1)
+                                   max_seq_len=args.max_seq_len, max_batch=1, cache_bits=args.cache_bits)
     else:
         engine = Engine.load(args.model, dtype=dtype, device=args.device,
-                             max_seq_len=args.max_seq_len, max_batch=1)
+                             max_seq_len=args.max_seq_len, max_batch=1, cache_bits=args.cache_bits)
     base = engine.default_sampling(args.sample, args.seed)
     sampling = SamplingParams(args.sample,
                               args.temperature if args.temperature is not None else base.temperature,

@@ -7,9 +7,11 @@ struct Kv4RowsArgs {
   const void* kv;          // [T, 2 nkv, D]: what is written, or (out) what is read
   void* out;
   const int* token_seq;    // [T]
-  const int* token_pos;    // [T]
+  const int* token_pos;    // [T], or null: a row is one of its sequence's newest tokens, by kv_len and cu_q
   const int* slots;        // [n_seqs]
   const int* block_table;  // [n_slots, max_pages]
+  const int* kv_len;       // [n_seqs]
+  const int* cu_q;         // [n_seqs + 1]
   uint8_t* pages;
   float* weights;          // [n_pages, nkv, 64] set to 0 for the tokens written, or null
   int T, n_seqs, n_slots, nkv, max_pages, n_pages;
@@ -17,9 +19,12 @@ struct Kv4RowsArgs {
 
 // Where token t of a step lives: its page (-1: nowhere) and its place there.
 __device__ __forceinline__ int find_token(const Kv4RowsArgs& a, int t, int& place) {
-  const int seq = a.token_seq[t], pos = a.token_pos[t];
+  const int seq = a.token_seq[t];
+  place = 0;
+  if ((unsigned)seq >= (unsigned)a.n_seqs) return -1;
+  const int pos = a.token_pos ? a.token_pos[t] : a.kv_len[seq] - (a.cu_q[seq + 1] - t);
+  if (pos < 0) return -1;
   place = pos & (KV4_PAGE - 1);
-  if ((unsigned)seq >= (unsigned)a.n_seqs || pos < 0) return -1;
   const int slot = a.slots[seq];
   if ((unsigned)slot >= (unsigned)a.n_slots) return -1;
   return kv4_page(a.block_table + (size_t)slot * a.max_pages, pos / KV4_PAGE, a.max_pages, a.n_pages);
@@ -185,6 +190,7 @@ static int rows(const Kv4RowsArgs* a, int D, int f32, bool write, cudaStream_t s
   if (a->T < 0 || a->nkv <= 0 || a->max_pages <= 0 || a->n_pages <= 0 || a->n_seqs < 0 || a->n_slots < 0 || !a->pages ||
       a->T > 0x7fffff00 || a->nkv > 0x100000)
     return GB_ERR_BAD_ARG;
+  if (!a->token_pos && (!a->kv_len || !a->cu_q)) return GB_ERR_BAD_ARG;
   if (((uintptr_t)(write ? a->kv : a->out) | (uintptr_t)a->pages) & 15) return GB_ERR_BAD_ARG;
   if (a->T == 0) return 0;
   if (D == 64) return f32 ? launch_rows<float, 64>(*a, write, s) : launch_rows<bf16, 64>(*a, write, s);

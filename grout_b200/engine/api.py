@@ -79,11 +79,13 @@ class Engine:
 
     # -- construction --------------------------------------------------------
     @classmethod
-    def _build(cls, arch, config, source, dtype, device, products=None, **kw) -> "Engine":
+    def _build(cls, arch, config, source, dtype, device, products=None, cache_bits=None, cache_weights=False,
+               **kw) -> "Engine":
         dtype, device = _dtype(dtype), _device(device)
         torch.cuda.set_device(device)
         plan = arch.plan(config)
-        model = Model(plan, BuildContext(dtype, device, products or ProductChoice()))
+        model = Model(plan, BuildContext(dtype, device, products or ProductChoice(), cache_bits, bool(cache_weights)))
+        model.check_cache()
         get = load_params(model.expected(), source, dtype, device)
         with torch.cuda.device(device):
             model.load(get)
@@ -95,12 +97,17 @@ class Engine:
     @classmethod
     def load(cls, model_dir: str, dtype="bfloat16", device="cuda:0", *, max_tokens=None,
              max_batch: int = 64, max_seq_len=None, use_graphs=None,
-             products: Optional[ProductChoice] = None) -> "Engine":
+             products: Optional[ProductChoice] = None, cache_bits: Optional[int] = None,
+             cache_weights: bool = False) -> "Engine":
         """A model folder: config.json chooses the architecture, the safetensors
         file(s) give the weights.  ``products`` names the kernels of the linear
-        layers (``parts.ProductChoice``; None: the defaults)."""
+        layers (``parts.ProductChoice``; None: the defaults).  ``cache_bits`` 4: keys and values
+        are kept in 4 bits (attention with heads of 64 or 128), 3.56 times as many tokens in the memory
+        of a bfloat16 cache; ``cache_weights``: and beside them the attention that every token has
+        been paid, for ``evict``."""
         arch, config = load_config(model_dir)
         return cls._build(arch, config, FolderSource(model_dir), dtype, device, products=products,
+                          cache_bits=cache_bits, cache_weights=cache_weights,
                           max_tokens=max_tokens, max_batch=max_batch, max_seq_len=max_seq_len,
                           use_graphs=use_graphs,
                           generation_config=GenerationConfig.from_model_dir(model_dir))
@@ -157,6 +164,24 @@ class Engine:
     def length(self, slot: int) -> int:
         return self.cache.length[slot]
 
+    def evict(self, slots: Sequence[int], keep: int, recent: int, first: int = 0) -> None:
+        """Cuts sequences of more than ``keep`` tokens to ``keep``: their ``first`` and ``recent`` newest tokens and of
+        the others those that were paid the most attention, by every kv head of every layer for itself (engines with
+        ``cache_bits=4, cache_weights=True``).  What follows goes on at its own position.  Weights are the attention of
+        every single token's step and of a prompt step's last rows (``parts.mixer.WEIGHED_ROWS``)."""
+        with torch.cuda.device(self.device):
+            self.cache.evict(slots, keep, recent, first)
+
+    def _entry(self, slot: int, toks):
+        ahead = self.cache.dropped.get(slot, 0)
+        return (slot, self.cache.length[slot], toks, ahead) if ahead else (slot, self.cache.length[slot], toks)
+
+    def _check_position(self, slot: int, n: int) -> None:
+        ahead = self.cache.dropped.get(slot, 0)
+        if ahead and ahead + self.cache.length[slot] + n > self.plan.max_position:
+            raise ValueError(f"a sequence of {ahead + self.cache.length[slot] + n} tokens, {ahead} of them let go of, exceeds "
+                             f"the architecture's {self.plan.max_position} positions")
+
     # -- the step --------------------------------------------------------------
     def step(self, entries: Sequence[Tuple[int, Sequence[int]]],
              want: Optional[Sequence[Sequence[int]]] = None) -> Optional[torch.Tensor]:
@@ -184,13 +209,15 @@ class Engine:
                 if not 0 <= int(p) < len(toks):
                     raise ValueError(f"wanted place {p} is outside the {len(toks)} tokens of entry {i}")
         for slot, toks in entries:
+            self._check_position(slot, len(toks))
+        for slot, toks in entries:
             self.cache.reserve(slot, len(toks))
         self.cache.flush()
-        packed = [(slot, self.cache.length[slot], list(toks)) for slot, toks in entries]
+        packed = [self._entry(slot, list(toks)) for slot, toks in entries]
         decode = all(len(t) == 1 for _s, t in entries)
         graph = None
         if self.use_graphs and decode:
-            graph = self.graphs.decode(len(entries), max(s + 1 for _slot, s, _t in packed))
+            graph = self.graphs.decode(len(entries), max(e[1] + 1 for e in packed))
         elif self.use_graphs:
             graph = self.graphs.prompt(sum(len(t) for _s, t in entries), len(entries),
                                        sum(len(w) for w in want))
@@ -265,10 +292,12 @@ class Engine:
         if not self.can_step_ahead(len(entries)):
             raise ValueError("this many sequences cannot step ahead: ask can_step_ahead first")
         for slot in slots:
+            self._check_position(slot, 1)
+        for slot in slots:
             self.cache.reserve(slot, 1)
         self.cache.flush()
         graph = self.graphs.decode(len(entries), max(self.cache.length[s] for s in slots) + 1)
-        packed = [(slot, self.cache.length[slot], [0]) for slot in slots]
+        packed = [self._entry(slot, [0]) for slot in slots]
         with torch.cuda.device(self.device):
             logits = graph.run(packed, tokens_from=(getattr(chosen, "dev", chosen),
                                                     [r for _s, r in entries]))

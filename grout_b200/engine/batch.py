@@ -66,7 +66,8 @@ def layout_sizes(n_tokens: int, n_seqs: int, n_want: int):
 
 def pack_step(entries: Sequence[Tuple[int, int, Sequence[int]]],
               want: Optional[Sequence[Sequence[int]]], pad_seqs: int = 0):
-    """entries: (slot, start, tokens) per sequence; want: per sequence the places
+    """entries: (slot, start, tokens) per sequence, or (slot, start, tokens, ahead) where the
+    positions run ``ahead`` of the places in the cache (tokens have been let go of); want: per sequence the places
     among its tokens whose logits are asked for.  ``pad_seqs`` appends sequences
     of one token with slot -1, which compute nothing that is kept.
     Returns (flat int32 array, meta dict)."""
@@ -85,11 +86,12 @@ def pack_step(entries: Sequence[Tuple[int, int, Sequence[int]]],
     slots = [e[0] for e in entries] + [-1] * pad_seqs
     starts = [e[1] for e in entries] + [0] * pad_seqs
     o = off["tokens"][0]
-    for i, (_slot, _start, toks) in enumerate(entries):
-        buf[o + cu[i]: o + cu[i + 1]] = np.asarray(toks, dtype=np.int64)
+    for i, e in enumerate(entries):
+        buf[o + cu[i]: o + cu[i + 1]] = np.asarray(e[2], dtype=np.int64)
     seq = np.repeat(np.arange(n_seqs, dtype=np.int32), q_lens)
     buf[off["token_seq"][0]: off["token_seq"][0] + n_tokens] = seq
-    pos = np.arange(n_tokens, dtype=np.int64) - cu[:-1][seq] + np.asarray(starts, dtype=np.int64)[seq]
+    first = np.asarray([e[1] + (e[3] if len(e) > 3 else 0) for e in entries] + [0] * pad_seqs, dtype=np.int64)
+    pos = np.arange(n_tokens, dtype=np.int64) - cu[:-1][seq] + first[seq]
     buf[off["token_pos"][0]: off["token_pos"][0] + n_tokens] = pos
     buf[off["cu_q"][0]: off["cu_q"][0] + n_seqs + 1] = cu
     buf[off["slots"][0]: off["slots"][0] + n_seqs] = slots

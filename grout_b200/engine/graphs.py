@@ -165,7 +165,7 @@ class DecodeGraph(StepGraph):
         starts = [e[1] for e in entries]
         out["tokens"][:n_real] = [e[2][0] for e in entries]
         out["tokens"][n_real:] = 0
-        out["token_pos"][:n_real] = starts
+        out["token_pos"][:n_real] = [e[1] + (e[3] if len(e) > 3 else 0) for e in entries]
         out["token_pos"][n_real:] = 0
         out["slots"][:n_real] = [e[0] for e in entries]
         out["slots"][n_real:] = -1
@@ -178,7 +178,8 @@ class DecodeGraph(StepGraph):
         self._fill([])
 
     def run(self, entries, tokens_from=None) -> torch.Tensor:
-        """entries: (slot, start, [token]) of the live sequences, at most n.
+        """entries: (slot, start, [token]) of the live sequences, at most n (and how far their positions are ahead
+        of their places, where they are: ``pack_step``).
         Returns logits [n, vocab]; rows beyond the live sequences are padding.
         The tensor is the graph's own and the next replay rewrites it.
         ``tokens_from`` = (int32 device tensor, rows): the token of entry k is

@@ -9,7 +9,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 
 import torch
 
-from ..cache import CacheLayout, SequenceCache
+from ..cache import CacheLayout, SequenceCache, StateSpec
 from ..parts.base import BuildContext, ParamSpec, Part, build_part
 from ..parts.norm import Averaged, HyperConnected, with_offset
 from ..parts.plan import ModelPlan
@@ -92,6 +92,21 @@ class Model:
                 specs.append(None if e.cache_of is not None else self.blocks[e.layer].cache_spec())
             self._layout = CacheLayout.from_specs(specs)
         return self._layout
+
+    def check_cache(self) -> None:
+        """Raises ValueError unless the layers' caches can be what the context asks for."""
+        bits, weights = self.ctx.cache_bits, self.ctx.cache_weights
+        if bits not in (None, 4):
+            raise ValueError(f"a cache of {bits} bits: 4, or None for the engine's type")
+        if weights and (bits is None or self.ctx.dtype != torch.bfloat16):
+            raise ValueError("weights of the tokens are kept beside a cache in 4 bits by a bfloat16 engine")
+        if bits is None:
+            return
+        for spec, layers in self.cache_layout().groups:
+            for s in getattr(spec, "specs", (spec,)):
+                if not isinstance(s, StateSpec) and getattr(s, "bits", None) != bits:
+                    raise ValueError(f"layers {layers} keep {s}, which has no form in {bits} bits: that is for grouped-query "
+                                     f"attention over keys and values of its own with heads of 64 or 128")
 
     def kernel_modules(self) -> Tuple[str, ...]:
         mods: List[str] = []

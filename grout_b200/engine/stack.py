@@ -76,6 +76,7 @@ def _plain_rotation(position) -> bool:
 
 def _plain_attention(m) -> bool:
     return (type(m) is GQAAttention and _as_it_is(m) and m.D == m.Dv == m.Ds == HEAD and _plain_rotation(m.position)
+            and m.kv_bits is None
             and m.window is None and not m.chunk and not m.keep_first and m.softcap is None and m.sink is None
             and not m.head_gate and not m.beside and not m.shares_kv and not m.values_are_keys
             and not m.conv_path and m.taps == 1 and m.q_temp is None

@@ -1863,32 +1863,40 @@ def _launch(dev: int, what: str, kernels: int, fn, *args) -> None:
     _check(rc, what, kernels)
 
 
-_KV4_ROWS = struct.Struct("@8P6i")
+_KV4_ROWS = struct.Struct("@10P6i")
 
 
-def _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page: int):
+def _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page: int, kv_len=None, cu_q=None):
     """What reading and writing rows share: (device, kv heads, D, rows, the arguments behind the rows' two addresses)."""
     dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
-    seq, pos = _take(token_seq, "token_seq", _I32, 1, dev), _take(token_pos, "token_pos", _I32, 1, dev)
+    seq, pos, lens, cu = _take(token_seq, "token_seq", _I32, 1, dev), 0, 0, 0
     sl, table = _take(slots, "slots", _I32, 1, dev), _take(block_table, "block table", _I32, 2, dev)
-    T = token_seq.shape[0]
-    if token_pos.shape[0] != T:
-        raise KernelError(f"{T} tokens have {token_pos.shape[0]} positions")
+    T, n_seqs = token_seq.shape[0], slots.shape[0]
+    if token_pos is not None:
+        pos = _take(token_pos, "token_pos", _I32, 1, dev)
+        if token_pos.shape[0] != T:
+            raise KernelError(f"{T} tokens have {token_pos.shape[0]} positions")
+    else:
+        lens, cu = _take(kv_len, "kv_len", _I32, 1, dev), _take(cu_q, "cu_q", _I32, 1, dev)
+        if kv_len.shape[0] != n_seqs or cu_q.shape[0] != n_seqs + 1:
+            raise KernelError("cu_q, slots and kv_len do not describe one list of sequences")
     w = 0 if weights is None else _take_weights(weights, n_pages, nkv, dev)
     n_slots, max_pages = block_table.shape
-    return dev, nkv, D, T, (seq, pos, sl, table, p, w, T, slots.shape[0], n_slots, nkv, max_pages, n_pages)
+    return dev, nkv, D, T, (seq, pos, sl, table, lens, cu, p, w, T, n_seqs, n_slots, nkv, max_pages, n_pages)
 
 
 @_profiled("kv4_write", lambda out, kv, *a, **k: (_nbytes(kv) + kv.numel() * 9 // 16, 0))
 def kv4_write(kv: torch.Tensor, nkv: int, D: int, *, token_seq, token_pos, slots, block_table, pages, page: int,
-              weights: Optional[torch.Tensor] = None) -> None:
+              weights: Optional[torch.Tensor] = None, kv_len: Optional[torch.Tensor] = None,
+              cu_q: Optional[torch.Tensor] = None) -> None:
     """Stores the step's keys and values ``kv`` [T, 2 nkv, D] (keys first; bfloat16 or 32-bit) in a cache of 4 bits
-    (``kv4_pages``): token t at position ``token_pos[t]`` of its sequence's cache.  Every 64 elements x of a key or
+    (``kv4_pages``): token t at place ``token_pos[t]`` of its sequence's cache or, without ``token_pos``, the step's rows
+    as their sequences' newest tokens (``kv_len`` and ``cu_q`` of the step).  Every 64 elements x of a key or
     value become round((x - m) / s) with m their least, rounded down to bfloat16, and s a fifteenth of their range,
     rounded up; they are read as s c + m, at most s / 2 off.  64 elements of which one is not finite, or whose range
     bfloat16 does not hold, are read as NaN.  Rows of slot -1 and places outside the block table store nothing; two
     rows of one call must not have the same place.  ``weights`` (``kv4_weigh``): the new tokens' are set to 0."""
-    dev, n, d, T, rest = _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page)
+    dev, n, d, T, rest = _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page, kv_len, cu_q)
     if kv.dim() != 3 or (n, d) != (nkv, D) or kv.shape != (T, 2 * nkv, D):
         raise KernelError(f"kv rows are {tuple(kv.shape)} for pages of {n} kv heads of {d}, expected [{T}, {2 * nkv}, {D}]")
     f32 = _suffix(kv.dtype) == "f32"

@@ -68,10 +68,13 @@ class ProductChoice:
 
 @dataclass(frozen=True)
 class BuildContext:
-    """Where, in which precision and on which product kernels a part computes."""
+    """Where, in which precision and on which product kernels a part computes, and in how many bits (None: the
+    precision's) and with or without weights of the tokens the keys and values are kept."""
     dtype: torch.dtype            # torch.bfloat16 or torch.float32
     device: torch.device
     products: ProductChoice = ProductChoice()
+    cache_bits: Optional[int] = None
+    cache_weights: bool = False
 
 
 class Part:

@@ -28,6 +28,9 @@ from .linear import Linear
 from .position import PositionEncoding
 
 
+WEIGHED_ROWS = 32      # a prompt step's last rows whose attention counts for the weights of a sequence's tokens
+
+
 class Mixer(Part):
     family = "mixer"
 
@@ -164,6 +167,10 @@ class GQAAttention(Mixer):
             raise ValueError("biases and convolutions of q and k take a rotation (or no position encoding)")
         self.qkv = self.o = None
         self.q_norm_w = self.k_norm_w = None
+        # in 4 bits: keys and values are made beside the queries and stored by a kernel of their own, for layers whose
+        # cache has that form (another's is refused when the model is built: Model.check_cache)
+        self.kv_bits = 4 if ctx.cache_bits == 4 and self.Ds in (64, 128) and not self.conv_path else None
+        self.weighed = ctx.cache_weights and self.kv_bits is not None
 
     def children(self):
         return (self.position,)
@@ -231,13 +238,16 @@ class GQAAttention(Mixer):
             mods += ops.fast_attention_modules(self.Ds, self.nq, self.nkv)
         else:
             mods += ("attn_f32",)
+        if self.kv_bits:
+            mods += ("kv4_cache", "attn_kv4")
+            mods += ("attn_prefill_kv4",) if self.ctx.dtype == torch.bfloat16 else ()
         return mods
 
     def cache_spec(self):
         if self.shares_kv:
             return None
         kv = KVSpec(self.nkv, self.Ds, self.kept_window, keep_first=self.keep_first,
-                    chunk=self.chunk or None)
+                    chunk=self.chunk or None, bits=self.kv_bits, weighed=self.weighed)
         if self.taps == 1:
             return kv
         # what the convolution of a sequence's next token looks back to
@@ -315,9 +325,17 @@ class GQAAttention(Mixer):
                                   rot_scale=rot.amplitude if rot else 1.0)
             if rot is None:
                 q, _k = self.position.apply_qk(q, q[:, :0], step.token_pos)
+            if cache.spec.bits:
+                return self._attend_kv4(q.contiguous(), None, step, cache, seen)
             return ops.attention(q.contiguous(), cache.k_pages, cache.v_pages, cache.block_table, **seen)
         common = dict(q_w=self.q_norm_w, k_w=self.k_norm_w, eps=self.qk_norm_eps or 0.0,
                       values_are_keys=self.values_are_keys, token_seq=step.token_seq, token_pos=step.token_pos, slots=step.slots)
+        if fused and cache.spec.bits:
+            q, kv = ops.qk_prepare(qkv, self.nq, self.nkv, self.D, inv_freq=rot.inv_freq if rot else None,
+                                   rot_dim=rot.rot_dim if rot else 0, want_kv_out=True, v_dim=self.Dv, q_temp=self.q_temp,
+                                   interleaved=bool(rot and rot.interleaved), row_width=self.Ds,
+                                   rot_scale=rot.amplitude if rot else 1.0, **common)
+            return self._attend_kv4(q, kv, step, cache, seen)
         if fused:
             q, _ = ops.qk_prepare(qkv, self.nq, self.nkv, self.D,
                                   inv_freq=rot.inv_freq if rot else None,
@@ -333,11 +351,29 @@ class GQAAttention(Mixer):
             k, v = kv[:, :self.nkv], kv[:, self.nkv:]
             q, k = self.position.apply_qk(q, k, step.token_pos)
             kv = torch.cat([k, v], dim=1).contiguous()
+            if cache.spec.bits:
+                return self._attend_kv4(q.contiguous(), kv, step, cache, seen)
             ops.kv_write(kv, self.nkv, self.D, token_seq=step.token_seq, token_pos=step.token_pos,
                          slots=step.slots, block_table=cache.block_table, k_pages=cache.k_pages,
                          v_pages=cache.v_pages, page=cache.page)
             q = q.contiguous()
         return ops.attention(q, cache.k_pages, cache.v_pages, cache.block_table, **seen)
+
+
+    def _attend_kv4(self, q, kv, step, cache, seen):
+        """The same over a cache in 4 bits: the step's keys and values stored (None: another layer has), the attention,
+        and with weights what the rows pay to the tokens.  A token's place is counted from its sequence's end: where
+        tokens have been let go of it is not its position."""
+        if kv is not None:
+            ops.kv4_write(kv, self.nkv, self.Ds, token_seq=step.token_seq, token_pos=None, kv_len=step.kv_len, cu_q=step.cu_q,
+                          slots=step.slots, block_table=cache.block_table, pages=cache.pages, page=cache.page,
+                          weights=cache.weights)
+        if cache.weights is None:
+            return ops.attention_kv4(q, cache.pages, cache.block_table, **seen)
+        out, lse = ops.attention_kv4(q, cache.pages, cache.block_table, want_lse=True, **seen)
+        of = {k: v for k, v in seen.items() if k != "sinks"}
+        ops.kv4_weigh(q, lse, cache.pages, cache.weights, cache.block_table, last=0 if step.decode else WEIGHED_ROWS, **of)
+        return out
 
 
 @register_part("mixer", "differential_attention")
