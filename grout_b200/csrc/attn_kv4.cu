@@ -306,11 +306,34 @@ __device__ __forceinline__ float cluster_read(const float* here, int rank) {
 }
 
 // Element d of a row's head from its maximum, sum and accumulator: the sink joins, and the quotient is stored.
-__device__ __forceinline__ void finish_row(const Kv4AttnArgs& a, int seq, int h, int d, int D, float M, float L, float O) {
-  const size_t row = (size_t)seq * a.nq + h;
-  if (a.sinks && (unsigned)a.slots[seq] < (unsigned)a.n_slots && a.sinks[h] != -INFINITY) O *= add_sink(a.sinks[h], M, L);
-  reinterpret_cast<bf16*>(a.out)[row * D + d] = __float2bfloat16(L != 0.f ? O / L : 0.f);
+template <typename T>
+__device__ __forceinline__ void finish_row(const Kv4AttnArgs& a, int t, bool live, int h, int d, int D, float M, float L,
+                                           float O) {
+  const size_t row = (size_t)t * a.nq + h;
+  if (a.sinks && live && a.sinks[h] != -INFINITY) O *= add_sink(a.sinks[h], M, L);
+  reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(L != 0.f ? O / L : 0.f);
   if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// The splits of some heads of a row are a cluster: each has left its sums [heads][D] and (maximum, sum)s in its shared
+// memory and finishes a share of the elements from all of them.
+template <typename T>
+__device__ __forceinline__ void finish_cluster(const Kv4AttnArgs& a, const float* sums, const float2* ml, int t, bool live,
+                                               int h0, int heads, int D, int rank) {
+  cluster_barrier();
+  const int n = a.n_splits;
+  for (int i = threadIdx.x * n + rank; i < heads * D; i += blockDim.x * n) {
+    const int h = i / D, d = i % D;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+    for (int c = 0; c < n; ++c) M = fmaxf(M, cluster_read(&ml[h].x, c));
+    for (int c = 0; c < n; ++c) {
+      const float mc = cluster_read(&ml[h].x, c), f = mc == -INFINITY ? 0.f : exp2f(mc - M);
+      L += cluster_read(&ml[h].y, c) * f;
+      O += cluster_read(sums + i, c) * f;
+    }
+    finish_row<T>(a, t, live, h0 + h, d, D, M, L, O);
+  }
+  cluster_barrier();                                   // (nobody leaves while its sums are read)
 }
 
 // A block's part of a pair, for all its threads.
@@ -648,9 +671,8 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     }
     __syncthreads();
     const bool alone = done.n_pieces <= 1;             // the result is final
+    const bool live = (unsigned)a.slots[done.seq] < (unsigned)a.n_slots;
     if (a.shared == 2) {
-      // The splits of a pair are a cluster: each leaves its sums in its shared memory and finishes a share of the pair's
-      // elements from all of them.
       for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
         const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
         float O = 0.f;
@@ -658,20 +680,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
         for (int w = 0; w < C::WARPS; ++w) O += red_o[(w * 8 + h) * C::PITCH + place] * red_f[w * 8 + h];
         reinterpret_cast<float*>(smem)[i] = O;         // (the ring is done with)
       }
-      cluster_barrier();
-      const int n = a.n_splits;
-      for (int i = threadIdx.x * n + done.piece; i < heads * D; i += C::WARPS * 32 * n) {
-        const int h = i / D, d = i % D;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int c = 0; c < n; ++c) M = fmaxf(M, cluster_read(&red_h[h].x, c));
-        for (int c = 0; c < n; ++c) {
-          const float mc = cluster_read(&red_h[h].x, c), f = mc == -INFINITY ? 0.f : exp2f(mc - M);
-          L += cluster_read(&red_h[h].y, c) * f;
-          O += cluster_read(reinterpret_cast<float*>(smem) + i, c) * f;
-        }
-        finish_row(a, done.seq, h0 + h, d, D, M, L, O);
-      }
-      cluster_barrier();                               // (nobody leaves while its sums are read)
+      finish_cluster<bf16>(a, reinterpret_cast<const float*>(smem), red_h, done.seq, live, h0, heads, D, done.piece);
       break;
     }
     for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
@@ -681,7 +690,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
       for (int w = 0; w < C::WARPS; ++w) O += red_o[(w * 8 + h) * C::PITCH + place] * red_f[w * 8 + h];
       const float2 ml = red_h[h];
       if (alone) {
-        finish_row(a, done.seq, h0 + h, d, D, ml.x, ml.y, O);
+        finish_row<bf16>(a, done.seq, live, h0 + h, d, D, ml.x, ml.y, O);
       } else if (done.piece < a.n_splits) {            // (more than the caller's bound of the lengths allows: merged as NaN)
         const size_t row = (size_t)done.seq * a.nq + h0 + h;
         a.part_o[(row * a.n_splits + done.piece) * D + d] = O;
@@ -748,7 +757,7 @@ __global__ void kv4_merge_kernel(const Kv4AttnArgs a, int D, int per_group) {
 // One row, up to four query heads of a kv head and a split of the keys a block; a warp takes 32 keys at a time.
 // Scores: a lane has a key and multiplies its elements with the queries, which lie in shared memory.  Values: half a
 // warp has a key, a lane the elements of one word (D 64: a quarter).  32-bit throughout; the scores see a code as
-// 1 + c / 16 (its bits at the top of the mantissa) and start from minus the query's sum, as in kv4_scores.
+// (c - 8) / 16 (its bits at the top of 1's mantissa, less 1.5) and add m + 8 s times the query's sum.
 template <int D>
 __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4AttnArgs a) {
   using F = Kv4<D>;
@@ -758,6 +767,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
   __shared__ float p_s[KV4_F32_WARPS][32][HC];            // P of the warp's keys
   __shared__ float red_o[KV4_F32_WARPS][HC][D];
   __shared__ float red_ml[KV4_F32_WARPS][HC][2];
+  __shared__ float2 ml_s[HC];                             // of a split of a cluster
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = a.nq / a.nkv, hgroups = (G + HC - 1) / HC;
@@ -770,7 +780,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
   const Stretches list(pos, 32, a.window, a.keep_first, a.chunk);
   const int keep = a.window > 0 ? a.keep_first : 0;
   const int v_end = a.n_splits == 1 ? list.n : min(list.n, (split + 1) * a.per);
-  if (split > 0 && split * a.per >= list.n) return;
+  if (a.shared != 2 && split > 0 && split * a.per >= list.n) return;
   const bool alone = a.n_splits == 1 || list.n <= a.per;
   const int* table = a.block_table + (size_t)(live ? slot : 0) * a.max_pages;
   for (int i = threadIdx.x; i < HC * D; i += blockDim.x)
@@ -815,21 +825,21 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       for (int g = 0; g < NG; ++g) {
         float acc[HC];
 #pragma unroll
-        for (int h = 0; h < HC; ++h) acc[h] = -qsum_s[h][g];
+        for (int h = 0; h < HC; ++h) acc[h] = 0.f;
 #pragma unroll
         for (int n = 8 * g; n < 8 * g + 8; ++n) {
           const uint32_t w = codes[F::key_word(n)];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int at = ((e & 1) << 4) + ((e >> 1) << 2);
-            const float c = __uint_as_float(((at < 19 ? w << (19 - at) : w >> (at - 19)) & 0x00780000u) | 0x3f800000u);
+            const float c = __uint_as_float(((at < 19 ? w << (19 - at) : w >> (at - 19)) & 0x00780000u) | 0x3f800000u) - 1.5f;
 #pragma unroll
             for (int h = 0; h < HC; ++h) acc[h] = fmaf(q_s[h][8 * n + e], c, acc[h]);
           }
         }
-        const float sc = 16.f * kv4_s(pair[g]), mn = kv4_m(pair[g]);
+        const float sc = 16.f * kv4_s(pair[g]), mid = fmaf(0.5f, sc, kv4_m(pair[g]));
 #pragma unroll
-        for (int h = 0; h < HC; ++h) s[h] += fmaf(sc, acc[h], mn * qsum_s[h][g]);
+        for (int h = 0; h < HC; ++h) s[h] += fmaf(sc, acc[h], mid * qsum_s[h][g]);
       }
     }
     __syncwarp();                                          // the warp's P of the last keys has been read
@@ -886,6 +896,8 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
     if (lane == 0) red_ml[warp][h][0] = m[h], red_ml[warp][h][1] = l[h];
   }
   __syncthreads();
+  // keys beyond the caller's bound of the lengths make the row NaN (merged by the second kernel, pieces says so)
+  const bool beyond = a.shared == 2 && list.n > a.per * a.n_splits;
   for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
     const int head = i / D, d = i % D;
     float M = -INFINITY;
@@ -899,16 +911,19 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       O += red_o[w][head][d] * f;
     }
     const size_t at = (size_t)row * a.nq + h0 + head;
-    if (alone) {
-      if (a.sinks && live && a.sinks[h0 + head] != -INFINITY) O *= add_sink(a.sinks[h0 + head], M, L);
-      reinterpret_cast<float*>(a.out)[at * D + d] = L != 0.f ? O / L : 0.f;
-      if (a.lse && d == 0) a.lse[at] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+    if (a.shared == 2) {
+      q_s[head][d] = beyond ? __int_as_float(0x7fffffff) : O;           // (the queries are done with)
+      if (d == 0) ml_s[head] = make_float2(beyond ? 0.f : M, L);
+    } else if (alone) {
+      finish_row<float>(a, row, live, h0 + head, d, D, M, L, O);
     } else {
       a.part_o[(at * a.n_splits + split) * D + d] = O;
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.n_splits + split) * 2) = make_float2(M, L);
     }
   }
-  if (a.n_splits > 1 && split == 0 && threadIdx.x == 0) a.pieces[(size_t)row * gridDim.y + blockIdx.y] = max(1, (list.n + a.per - 1) / a.per);
+  if (a.shared == 2) finish_cluster<float>(a, &q_s[0][0], ml_s, row, live, h0, heads, D, split);
+  else if (a.n_splits > 1 && split == 0 && threadIdx.x == 0)
+    a.pieces[(size_t)row * gridDim.y + blockIdx.y] = max(1, (list.n + a.per - 1) / a.per);
 }
 
 // ---------------------------------------------------------------- the weights that tokens gather
@@ -1103,10 +1118,12 @@ GB_EXPORT int gb_attn_kv4_f32(const Kv4AttnArgs* a, int D, cudaStream_t s) {
       (long long)a->n_rows * a->nq > 0x7fffffffll)
     return GB_ERR_UNSUPPORTED;
   if (a->n_rows == 0) return 0;
+  if (a->shared && (a->shared != 2 || a->n_splits < 2 || a->n_splits > 8)) return GB_ERR_BAD_ARG;
   const dim3 grid((unsigned)(a->n_rows * a->n_splits), a->nkv * hgroups);
-  rc = D == 64 ? gb_launch(kv4_f32_kernel<64>, grid, dim3(KV4_F32_WARPS * 32), 0, s, *a)
-               : gb_launch(kv4_f32_kernel<128>, grid, dim3(KV4_F32_WARPS * 32), 0, s, *a);
-  if (rc || a->n_splits == 1) return rc;
+  const int cluster = a->shared == 2 ? a->n_splits : 1;
+  rc = D == 64 ? gb_launch_cluster(kv4_f32_kernel<64>, grid, dim3(KV4_F32_WARPS * 32), 0, s, cluster, *a)
+               : gb_launch_cluster(kv4_f32_kernel<128>, grid, dim3(KV4_F32_WARPS * 32), 0, s, cluster, *a);
+  if (rc || a->n_splits == 1 || cluster > 1) return rc;
   return gb_launch(kv4_merge_kernel<float>, dim3((unsigned)(a->n_rows * a->nq)), dim3(D), 0, s, *a, D, KV4_F32_HEADS);
 }
 

@@ -190,9 +190,9 @@ static int rows(const Kv4RowsArgs* a, int D, int f32, bool write, cudaStream_t s
   if (a->T < 0 || a->nkv <= 0 || a->max_pages <= 0 || a->n_pages <= 0 || a->n_seqs < 0 || a->n_slots < 0 || !a->pages ||
       a->T > 0x7fffff00 || a->nkv > 0x100000)
     return GB_ERR_BAD_ARG;
-  if (!a->token_pos && (!a->kv_len || !a->cu_q)) return GB_ERR_BAD_ARG;
   if (((uintptr_t)(write ? a->kv : a->out) | (uintptr_t)a->pages) & 15) return GB_ERR_BAD_ARG;
   if (a->T == 0) return 0;
+  if (!a->token_seq || !a->slots || !a->block_table || (!a->token_pos && (!a->kv_len || !a->cu_q))) return GB_ERR_BAD_ARG;
   if (D == 64) return f32 ? launch_rows<float, 64>(*a, write, s) : launch_rows<bf16, 64>(*a, write, s);
   if (D == 128) return f32 ? launch_rows<float, 128>(*a, write, s) : launch_rows<bf16, 128>(*a, write, s);
   return GB_ERR_UNSUPPORTED;

@@ -1941,11 +1941,13 @@ def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int)
     return splits, least, 2 if way == 2 and splits <= 8 else 0
 
 
-def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int]:
-    """(splits, stretches of 32 keys in a split) of the 32-bit kernel."""
+def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int, int]:
+    """(splits, stretches of 32 keys in a split, way) of the 32-bit kernel, ``way`` 0 or 2 as above: clusters while eight
+    splits of up to eight stretches do."""
     tiles = max(1, (keys + 31) // 32)
-    per = KV4_SPLIT_OVERRIDE or max(8, -(-tiles * pairs // (8 * sms)), -(-tiles // 64))
-    return -(-tiles // per), per
+    per = KV4_SPLIT_OVERRIDE or max(4, -(-tiles * pairs // (8 * sms)), -(-tiles // 8) if tiles <= 64 else -(-tiles // 64))
+    splits = -(-tiles // per)
+    return splits, per, 2 if 1 < splits <= 8 and KV4_SHARE_OVERRIDE in (None, 2) else 0
 
 
 def _kv4_query(q, pages, block_table, step, page: int, scale, softcap, window, keep_first, chunk):
@@ -2029,9 +2031,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     each = 4 if f32 else 8
     groups = nkv * ((nq // nkv + each - 1) // each)
     keys = _keys_visited(step.max_kv_len, window, page, keep_first, chunk)
-    way = 0
     if f32:
-        ns, per = kv4_split_plan_f32(T * groups, keys, sms)
+        ns, per, way = kv4_split_plan_f32(T * groups, keys, sms)
     else:
         ns, per, way = kv4_split_plan(n_seqs, n_seqs * groups, keys, max_pages, sms)
     po = pm = pc = 0
@@ -2045,7 +2046,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
                           nkv, max_pages, n_pages, window, ns, per, way, keep_first, chunk, scale_log2, cap_log2,
                           cap_inv)
     if f32:
-        _launch(dev, "attn_kv4_f32", 2 if ns > 1 else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
+        _launch(dev, "attn_kv4_f32", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
     else:
         _launch(dev, "attn_kv4_decode", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, KV4_PER_SM * sms)
     return (out, lse) if want_lse else out

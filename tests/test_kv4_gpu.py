@@ -219,10 +219,12 @@ def test_single_tokens(lens, nq, nkv, D, dtype, seen):
     attend(c, [1] * len(lens), nq, dtype, sinks=len(lens) % 2 == 1, pad=len(lens) % 3, **seen)
 
 
+@pytest.mark.parametrize("way", [0, 2])
 @pytest.mark.parametrize("stretches", [1, 3, 4, 8, 100])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_splits_of_the_keys(stretches, dtype, monkeypatch):
+def test_splits_of_the_keys(stretches, dtype, way, monkeypatch):
     monkeypatch.setattr(ops, "KV4_SPLIT_OVERRIDE", stretches)
+    monkeypatch.setattr(ops, "KV4_SHARE_OVERRIDE", way)
     c = Cache([1000, 1, 130], 2, 128, dtype)
     attend(c, [1, 1, 1], 8, dtype, sinks=True, pad=1)
     attend(c, [1, 1, 1], 8, dtype, window=200, keep_first=3)
