@@ -64,8 +64,14 @@ __device__ __forceinline__ bool find_row(const Kv4AttnArgs& a, int t, int& pos) 
 // ---------------------------------------------------------------- bfloat16, single tokens
 #define KV4_SHARED_SEQS 256      // the most sequences whose stretches are shared out (their counts lie beside four rings an SM)
 
-// before[i]: the stretches of the sequences in front of i (of one pair of each).  Returns how many stretches a block
-// takes.  For a whole block of 128 threads.
+// What beginning and ending a pair's part costs a block, in stretches: every pair counts as so many more, which come in
+// front of its own.  (A part more took a block 5.5 us where its stretches took 0.55 each.  60 sequences of up to 4,096
+// keys, 200 of up to 1,200, us: counted as none 58.5 and 73.0, six 53.7 and 64.2, ten 53.6 and 63.4, twenty 54.9 and 65.5.)
+#define KV4_PART_COST 10
+__device__ __forceinline__ int part_stretches(int n) { return n > 0 ? n + KV4_PART_COST : 0; }
+
+// before[i]: the stretches of the sequences in front of i (of one pair of each), their parts' cost included.  Returns how
+// many a block takes.  For a whole block of 128 threads.
 __device__ __forceinline__ unsigned share_out(const Kv4AttnArgs& a, int unit, int groups, int* before) {
   __shared__ int warp_sums[4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, each = (a.n_seqs + 127) / 128;
@@ -73,7 +79,7 @@ __device__ __forceinline__ unsigned share_out(const Kv4AttnArgs& a, int unit, in
   for (int i = tid * each; i < min(a.n_seqs, (tid + 1) * each); ++i) {
     int pos;
     find_row(a, i, pos);
-    mine += Stretches(pos, unit, a.window, a.keep_first, a.chunk).n;
+    mine += part_stretches(Stretches(pos, unit, a.window, a.keep_first, a.chunk).n);
   }
   int sum = mine;
 #pragma unroll
@@ -94,7 +100,7 @@ __device__ __forceinline__ unsigned share_out(const Kv4AttnArgs& a, int unit, in
     int pos;
     find_row(a, i, pos);
     before[i] = here;
-    here += Stretches(pos, unit, a.window, a.keep_first, a.chunk).n;
+    here += part_stretches(Stretches(pos, unit, a.window, a.keep_first, a.chunk).n);
   }
   if (tid == 0) before[a.n_seqs] = all;
   __syncthreads();
@@ -278,9 +284,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 // The blocks share out the stretches of 32 keys of all pairs (sequence, group of up to eight query heads of one kv head)
 // evenly, in the order of the pairs: a block has one run of them, which may end inside a pair and go on in the next, so
-// sequences of unequal lengths leave no SM waiting (60 sequences of 700 to 4,096 keys: SPLIT_US us with a fixed number of
-// keys a block, which the SMs were through with between 59 and 105 thousand cycles, SHARED_US so).  With one split a
-// block has a whole pair.
+// sequences of unequal lengths leave no SM waiting.  (With a fixed number of keys a block the SMs were through with 60
+// sequences of 700 to 4,096 keys after 59 to 105 thousand cycles.)  Where the splits fit the GPU at once they are fixed
+// instead, a block each, and up to eight of a pair are a cluster that puts its results together; with one split a block
+// has a whole pair.
 // Of a run's part of a pair every warp takes stretches in turn, each through a ring of its own that bulk copies fill,
 // and keeps its own maximum, sum and accumulator: no barrier of the block lies in the loop.  For the two records of a
 // stretch
@@ -293,6 +300,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // below 2^8, so it stays below 2^15 and what it loses at the other end is below 2^-25 of a whole probability.  Values
 // are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range; m + 8 s times P
 // is summed in 32 bits.
+// What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 404 of them, 288 of which are
+// its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products); four warps
+// a scheduler issue on 61 % of the cycles, the logical pipe is busy for half of them, and the memory gives 3.2 TB/s of 6.45
+// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 53.6 us, 26.7 at the memory's rate).  Three blocks an SM with
+// 168 registers and no spills are no faster.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -378,7 +390,13 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x)      // sequences without keys have nobody else
       if (before[i + 1] == before[i]) empty_row(a, i, groups, D);
     seq_next = find_stretch(before, a.n_seqs, at / groups);
-    more = at < end;
+    if (at < end) {
+      // (a run that lies in a pair's cost, but for its end, has nothing to do)
+      const unsigned first = (unsigned)before[seq_next] * groups, whole = (unsigned)(before[seq_next + 1] - before[seq_next]);
+      more = end > first + (at - first) / whole * whole + KV4_PART_COST;
+    } else {
+      more = false;
+    }
   }
   if (!more) return;
 
@@ -422,15 +440,16 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     const Stretches list(pos, C::UNIT, BOUNDED ? a.window : 0, BOUNDED ? a.keep_first : 0, BOUNDED ? a.chunk : 0);
     int v_begin, v_end;
     if (a.shared == 1) {
-      const unsigned first = (unsigned)before[part.seq] * groups, n = (unsigned)list.n;
-      part.group = (int)((at - first) / n);
-      const unsigned pair = first + part.group * n, piece0 = pair / run;
-      v_begin = (int)(at - pair);
-      v_end = (int)min(n, v_begin + (end - at));
+      // the pair's own stretches are [pair, pair + n) of the list, behind its cost
+      const unsigned first = (unsigned)before[part.seq] * groups, n = (unsigned)list.n, whole = n + KV4_PART_COST;
+      part.group = (int)((at - first) / whole);
+      const unsigned pair = first + part.group * whole + KV4_PART_COST, piece0 = pair / run;
+      v_begin = (int)(max(at, pair) - pair);
+      v_end = (int)min(n, end - pair);
       part.piece = (int)(blockIdx.x - piece0);
       part.n_pieces = (int)((pair + n - 1) / run - piece0) + 1;
-      at += v_end - v_begin;
-      more = at < end;
+      at = pair + v_end;
+      more = at < end && end - at > KV4_PART_COST;      // (and not only a next pair's cost)
       if (at == (unsigned)before[part.seq + 1] * groups && more)
         do ++seq_next; while (before[seq_next + 1] == before[seq_next]);      // (there is one with keys)
     } else {
@@ -1091,7 +1110,7 @@ static int decode(const Kv4AttnArgs& a, int blocks, cudaStream_t s) {
   // (all stretches are counted in 32 bits, and a block's run may reach beyond them)
   if (a.shared == 2 && (a.n_splits < 2 || a.n_splits > 8)) return GB_ERR_BAD_ARG;
   if (a.shared == 1 && (a.n_splits < 2 || a.n_seqs > KV4_SHARED_SEQS || blocks <= 0 ||
-                   pairs * (4ll * a.max_pages + 4) + 2ll * blocks * a.per > 0x7fffffffll))
+                   pairs * (4ll * a.max_pages + 64) + 2ll * blocks * a.per > 0x7fffffffll))
     return GB_ERR_BAD_ARG;
   const unsigned grid = (unsigned)(a.shared == 1 ? blocks : pairs * a.n_splits);
   const int rc = a.window > 0 || a.chunk > 0 ? decode_launch<D, true>(a, grid, s) : decode_launch<D, false>(a, grid, s);

@@ -24,8 +24,9 @@ struct Kv4Pages {
   __device__ __forceinline__ static void before_padding() { pdl_wait(); }
   __device__ __forceinline__ static void prepare(const Params&) {}
   // C tanh(x) log2 e = C log2 e (1 - 2 / (2^(2 x log2 e) + 1)) with the special unit's power and inverse as they are
-  // (2^-22 of their size off; no power is 0 and an infinite one's inverse is 0, which are the two ends) and two scores
-  // to an instruction around them.  CAP_US
+  // (2^-22 of their size off; an exponent too small gives 0 and an infinite power's inverse is 0, which are the two
+  // ends) and two scores to an instruction around them: six sequences' chunks of up to 384 rows, windowed, 20 heads of
+  // 64, take 74.2 us, 83.0 with the powers and quotients of the 16-bit kernel, 48.1 without a cap.
   __device__ __forceinline__ static void cap_scores(float (&s)[AT_BN], const ScoreCap& cap) {
     const float in = cap.cap_inv * 2.8853900817779268f;
     const uint64_t in2 = pack_f32x2(in, in), zero2 = pack_f32x2(0.f, 0.f), one2 = pack_f32x2(1.f, 1.f);

@@ -1936,7 +1936,7 @@ def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int)
         return 1, tiles, 0
     if way is None:
         way = 1 if splits * pairs > blocks else 2 if splits <= 8 else 0
-    if way == 1 and n_seqs <= 256 and pairs * (4 * max_pages + 4) + 2 * blocks * least <= 0x7fffffff:
+    if way == 1 and n_seqs <= 256 and pairs * (4 * max_pages + 64) + 2 * blocks * least <= 0x7fffffff:
         return min(blocks, splits + 1), least, 1
     return splits, least, 2 if way == 2 and splits <= 8 else 0
 
