@@ -1938,6 +1938,10 @@ def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int)
         way = 1 if splits * pairs > blocks else 2 if splits <= 8 else 0
     if way == 1 and n_seqs <= 256 and pairs * (4 * max_pages + 64) + 2 * blocks * least <= 0x7fffffff:
         return min(blocks, splits + 1), least, 1
+    if way == 1:             # (too many to share out: no more splits than two waves of blocks)
+        splits = min(splits, -(-2 * blocks // pairs))
+        least = -(-tiles // splits)
+        splits = -(-tiles // least)
     return splits, least, 2 if way == 2 and splits <= 8 else 0
 
 

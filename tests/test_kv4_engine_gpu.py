@@ -210,3 +210,55 @@ def test_positions_end_where_the_architecture_does():
     with pytest.raises(ValueError):
         eng.step([(s, [1])])
     assert eng.length(s) == 60
+
+
+# ---------------------------------------------------------------- the other designs
+def _designs():
+    from test_kakotar_engine_gpu import YARN, _att, _light, _rot
+    from test_mananex_engine_gpu import MAN
+    from test_sonalorn_engine_gpu import _attn, _delta
+    from test_suvazen_engine_gpu import SUV
+    # rotations, caps, sinks, windows, loops and values that are the unrotated keys; kept first keys and head gates beside
+    # a state; a layer that reads another's keys; a query temperature and values narrower than the keys
+    return {
+        "suvazen": SUV["R"], "mananex": MAN["Q"],
+        "kakotar": dict(architecture="Kakotar", vocab=300, width=128, norm={"eps": 3e-6}, layers=[
+            dict(type="attention", mixer=_att(4, 2, 64, 64, 0.3, 70, _rot(1e5, 32, YARN)), mlp=None),
+            dict(type="lightning", mixer=_light(2, 16, 16, 0.5, 0.9), mlp=None),
+            dict(type="attention", mixer=_att(8, 2, 64, 64, 0.25, 40, _rot(1e5, 32, YARN), kv_from=0), mlp=None)]),
+        "sonalorn": dict(architecture="Sonalorn", vocab=200, width=96, max_positions=512, norm={"eps": 1e-5}, layers=[
+            dict(type="delta", mixer=_delta(heads=2, kv_heads=2, dim=32, vdim=32, conv=4), mlp=None),
+            dict(type="attention", mixer=_attn(heads=4, kv_heads=1, dim=64, vdim=40, scale=0.15), mlp=None)])}
+
+
+@pytest.mark.parametrize("name", ["suvazen", "mananex", "kakotar", "sonalorn"])
+def test_the_other_designs(name, monkeypatch):
+    """In 32 bits, against the same engine with a 32-bit cache whose keys and values pass through the plain 4-bit form
+    in front of every attention: the same keys, so the logits differ by the attention kernels' 32-bit sums."""
+    config = _designs()[name]
+    tokens = random_tokens(170, 150, 4)
+    eng = Engine.random(config, 3, dtype="float32", max_tokens=4096, max_batch=4, cache_bits=4, use_graphs=False)
+    rows = [run_whole(eng, tokens), run_tail_decoded(eng, tokens, 50)]
+    usual = ops.attention
+
+    def through(q, k_pages, v_pages, *a, **kw):
+        f = lambda x: kv4.value(*kv4.quantise(x.cpu())).to(x.device)
+        return usual(q, f(k_pages), f(v_pages), *a, **kw)
+    oracle = Engine.random(config, 3, dtype="float32", max_tokens=512, max_batch=4, use_graphs=False)
+    with monkeypatch.context() as m:
+        m.setattr(ops, "attention", through)
+        want = run_whole(oracle, tokens)
+    spread = float((want - want.mean(-1, keepdim=True)).pow(2).mean().sqrt())
+    for got in rows:
+        assert float((got - want).abs().max()) < 1e-3 * spread, float((got - want).abs().max()) / spread
+    # (it does matter: without the 4-bit form the logits are elsewhere)
+    plain = run_whole(oracle, tokens)
+    assert float((plain - want).abs().max()) > 0.01 * spread
+
+
+def test_designs_without_the_form():
+    from test_keralix_engine_gpu import KER
+    from test_zutazen_engine_gpu import ZUT
+    for config in (next(iter(KER.values())), next(iter(ZUT.values()))):
+        with pytest.raises(ValueError, match="4 bits"):
+            Engine.random(config, 3, max_tokens=512, max_batch=4, cache_bits=4)
