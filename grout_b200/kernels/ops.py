@@ -1853,14 +1853,23 @@ def _take_weights(weights, n_pages: int, nkv: int, dev: int) -> int:
     return p
 
 
-def _launch(dev: int, what: str, kernels: int, fn, *args) -> None:
-    """Calls a kernel's entry point on the current stream of device ``dev``."""
-    if torch._C._cuda_getDevice() == dev:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
+def _launch(dev: int, what: str, kernels: int, cost, fn, *args) -> None:
+    """Calls a kernel's entry point on the current stream of device ``dev``; with a profile on, as ``_profiled`` does,
+    between two events and with its ``cost`` (bytes, flops) noted."""
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            return _launch(dev, what, kernels, cost, fn, *args)
+    prof = _PROFILE
+    if prof is None:
+        return _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), what, kernels)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    if prof.lead_us:
+        _fn("elementwise", "gb_delay_ns", "lp")(prof.lead_us * 1000, _stream())
+    a.record()
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    b.record()
     _check(rc, what, kernels)
+    prof.add(what, a, b, *cost)
 
 
 _KV4_ROWS = struct.Struct("@10P6i")
@@ -1885,7 +1894,6 @@ def _kv4_rows(pages, weights, token_seq, token_pos, slots, block_table, page: in
     return dev, nkv, D, T, (seq, pos, sl, table, lens, cu, p, w, T, n_seqs, n_slots, nkv, max_pages, n_pages)
 
 
-@_profiled("kv4_write", lambda out, kv, *a, **k: (_nbytes(kv) + kv.numel() * 9 // 16, 0))
 def kv4_write(kv: torch.Tensor, nkv: int, D: int, *, token_seq, token_pos, slots, block_table, pages, page: int,
               weights: Optional[torch.Tensor] = None, kv_len: Optional[torch.Tensor] = None,
               cu_q: Optional[torch.Tensor] = None) -> None:
@@ -1901,10 +1909,10 @@ def kv4_write(kv: torch.Tensor, nkv: int, D: int, *, token_seq, token_pos, slots
         raise KernelError(f"kv rows are {tuple(kv.shape)} for pages of {n} kv heads of {d}, expected [{T}, {2 * nkv}, {D}]")
     f32 = _suffix(kv.dtype) == "f32"
     src = _take16(kv, "kv rows", kv.dtype, 3, dev)
-    _launch(dev, "kv4_write", 1 if T else 0, _fn("kv4_cache", "gb_kv4_write", "piip"), _KV4_ROWS.pack(src, 0, *rest), D, f32)
+    cost = _PROFILE and (_nbytes(kv) + kv.numel() * 9 // 16, 0)
+    _launch(dev, "kv4_write", 1 if T else 0, cost, _fn("kv4_cache", "gb_kv4_write", "piip"), _KV4_ROWS.pack(src, 0, *rest), D, f32)
 
 
-@_profiled("kv4_read", lambda out, pages, **k: (_nbytes(out) + out.numel() * 9 // 16, 0))
 def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, page: int,
              dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The keys and values [T, 2 nkv, D] that a 4-bit cache holds at the given places, as ``kv4_write`` takes them
@@ -1913,7 +1921,8 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
     dev, nkv, D, T, rest = _kv4_rows(pages, None, token_seq, token_pos, slots, block_table, page)
     f32 = _suffix(dtype) == "f32"
     out = pages.new_empty((T, 2 * nkv, D), dtype=dtype)
-    _launch(dev, "kv4_read", 1 if T else 0, _fn("kv4_cache", "gb_kv4_read", "piip"),
+    cost = _PROFILE and (_nbytes(out) + out.numel() * 9 // 16, 0)
+    _launch(dev, "kv4_read", 1 if T else 0, cost, _fn("kv4_cache", "gb_kv4_read", "piip"),
             _KV4_ROWS.pack(0, out.data_ptr(), *rest), D, f32)
     return out
 
@@ -1994,17 +2003,10 @@ def _kv4_query(q, pages, block_table, step, page: int, scale, softcap, window, k
         window, keep_first, chunk, scale * _LOG2E, softcap * _LOG2E, scale / softcap if softcap else 0.0)
 
 
-def _cost_attention_kv4(out, q, pages, block_table, *, step, window=None, chunk=0, **kw):
-    out = out[0] if isinstance(out, tuple) else out
-    return _attention_cost(out, q, pages.shape[1] * pages.shape[3] // 16, kv_len=step.kv_len, slots=step.slots,
-                           cu_q=step.cu_q, window=window, chunk=chunk)
-
-
 _KV4_ATTN = struct.Struct("@14P13i3f")
 _KV4_PROMPT = struct.Struct("@6P6ifP2f3i")
 
 
-@_profiled("attention_kv4", _cost_attention_kv4)
 def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, *, step, page: int, scale: float,
                   window: Optional[int] = None, softcap: Optional[float] = None,
                   sinks: Optional[torch.Tensor] = None, keep_first: int = 0, chunk: int = 0, want_lse: bool = False):
@@ -2031,6 +2033,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     err = _TC_ERRORS.get(dev)
     err = (_tc_error_flag(q.device) if err is None else err).data_ptr()
     sms = _SM_COUNT.get(dev) or _sm_count(q.device)
+    cost = _PROFILE and _attention_cost(out, q, nkv * 9 * D // 8, kv_len=step.kv_len, slots=step.slots, cu_q=step.cu_q,
+                                        window=window, chunk=chunk)
     if not (f32 or step.decode):
         pack, rows = prefill_tc_plan(lambda n: _q_blocks(step.q_lens, None, n, T, n_seqs), nq, nkv, sms)
         blocks = _q_blocks(step.q_lens, None, rows // pack, T, n_seqs)
@@ -2039,7 +2043,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
             blocks = _q_blocks(step.q_lens, None, rows // pack, T, n_seqs)
         args = _KV4_PROMPT.pack(table, cu, sl, lens, out.data_ptr(), err, n_seqs, nq, nkv, max_pages, window, blocks,
                                 scale_log2, sk, cap_log2, cap_inv, keep_first, chunk, pack)
-        _launch(dev, "attn_prefill_kv4", 1, _fn("attn_prefill_kv4", "gb_attn_prefill_kv4", "ppppiiiiip"), qp, p, args, lp, T,
+        _launch(dev, "attn_prefill_kv4", 1, cost, _fn("attn_prefill_kv4", "gb_attn_prefill_kv4", "ppppiiiiip"), qp, p, args, lp, T,
                 n_pages, n_slots, D, rows)
         return (out, lse) if want_lse else out
     seq = 0
@@ -2065,16 +2069,15 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
                           nkv, max_pages, n_pages, window, ns, per, way, keep_first, chunk, scale_log2, cap_log2,
                           cap_inv)
     if f32:
-        _launch(dev, "attn_kv4_f32", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
+        _launch(dev, "attn_kv4_f32", 2 if po else 1, cost, _fn("attn_kv4", "gb_attn_kv4_f32", "pip"), args, D)
     else:
-        _launch(dev, "attn_kv4_decode", 2 if po else 1, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, KV4_PER_SM * sms)
+        _launch(dev, "attn_kv4_decode", 2 if po else 1, cost, _fn("attn_kv4", "gb_attn_kv4_decode", "piip"), args, D, KV4_PER_SM * sms)
     return (out, lse) if want_lse else out
 
 
 _KV4_WEIGH = struct.Struct("@8P11i3f")
 
 
-@_profiled("kv4_weigh", lambda out, q, lse, *a, **k: (_nbytes(q, lse), 0))
 def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, *,
               step, page: int, scale: float, window: Optional[int] = None, softcap: Optional[float] = None,
               keep_first: int = 0, chunk: int = 0, last: int = 0) -> None:
@@ -2100,13 +2103,15 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
     blocks = max(1, min(-(-step.max_kv_len // 128), -(-8 * sms // max(1, nkv * n_seqs))))
     args = _KV4_WEIGH.pack(qp, lp, p, w, table, sl, lens, cu, T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window,
                            keep_first, chunk, int(last), scale_log2, cap_log2, cap_inv)
-    _launch(dev, "kv4_weigh", 1 if T else 0, _fn("attn_kv4", "gb_kv4_weigh", "piip"), args, D, blocks)
+    # (the keys with their pairs, and the weights in and out)
+    cost = _PROFILE and _attention_cost(lse, q, nkv * (5 * D // 8 + 8), kv_len=step.kv_len, slots=step.slots, cu_q=step.cu_q,
+                                        window=window, chunk=chunk)
+    _launch(dev, "kv4_weigh", 1 if T else 0, cost, _fn("attn_kv4", "gb_kv4_weigh", "piip"), args, D, blocks)
 
 
 _KV4_CHOOSE, _KV4_MOVE = struct.Struct("@6P8i"), struct.Struct("@8P8i")
 
 
-@_profiled("kv4_evict", lambda out, pages, *a, **k: (2 * out[0].numel() * (pages.shape[3] // 16 + 4), 0))
 def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, *, slots: torch.Tensor,
               kv_len: torch.Tensor, page: int, keep: int, recent: int, first: int = 0,
               into: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -2142,15 +2147,16 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
                               keep, recent, first)
     rest = (sl, kept.data_ptr(), n_seqs, n_slots, nkv, n_pages, keep)
     evict = _fn("kv4_cache", "gb_kv4_evict", "pppip")
+    cost = _PROFILE and (2 * kept.numel() * (pages.shape[3] // 16 + 4), 0)
     if to_table != table:
-        _launch(dev, "kv4_evict", 2, evict, choose, _KV4_MOVE.pack(p, p, w, w, table, to_table, *rest, max_pages, to_max, 0),
+        _launch(dev, "kv4_evict", 2, cost, evict, choose, _KV4_MOVE.pack(p, p, w, w, table, to_table, *rest, max_pages, to_max, 0),
                 None, D)
     else:      # by way of memory of this call's own: tokens move within the pages that others are read from
         records = (keep + 15) // 16
         held = torch.empty((n_seqs, nkv, records, pages.shape[3]), dtype=torch.uint8, device=pages.device)
         w_held = torch.empty((n_seqs, nkv, records * 16), dtype=_F32, device=pages.device)
         h, wh = held.data_ptr(), w_held.data_ptr()
-        _launch(dev, "kv4_evict", 3, evict, choose, _KV4_MOVE.pack(p, h, w, wh, table, 0, *rest, max_pages, 0, 0),
+        _launch(dev, "kv4_evict", 3, cost, evict, choose, _KV4_MOVE.pack(p, h, w, wh, table, 0, *rest, max_pages, 0, 0),
                 _KV4_MOVE.pack(h, p, wh, w, 0, table, *rest, 0, max_pages, 1), D)
     return kept, new
 

@@ -623,3 +623,23 @@ def test_refusals():
         raise AssertionError(f"call {i} was not refused")
     assert torch.equal(c.pages, before)
     torch.cuda.synchronize()
+
+
+def test_the_profile_knows_the_operators():
+    c = Cache([200, 30], 2, 64, weights=True)
+    step, q = c.step([1, 1]), queries(2, 8, 64, torch.bfloat16, 0).to(DEV)
+    prof = ops.OpProfile()
+    ops.set_profile(prof)
+    try:
+        out, lse = ops.attention_kv4(q, c.pages, c.table, step=step, page=64, scale=0.1, want_lse=True)
+        ops.kv4_weigh(q, lse, c.pages, c.weights, c.table, step=step, page=64, scale=0.1)
+        ops.kv4_read(c.pages, token_seq=ints(0), token_pos=ints(3), **c.at)
+        ops.kv4_write(c.kv[:1].to(DEV), 2, 64, token_seq=ints(0), token_pos=ints(3), pages=c.pages, **c.at)
+        ops.kv4_evict(c.pages, c.weights, c.table, slots=ints(*c.slots), kv_len=ints(200, 30), page=64, keep=50, recent=5)
+    finally:
+        ops.set_profile(None)
+    totals = prof.totals()
+    assert {"attn_kv4_decode", "kv4_weigh", "kv4_read", "kv4_write", "kv4_evict"} == set(totals)
+    # 230 tokens of two heads of 72 bytes for keys and as many for values; eight heads in and out; 4 D flops a pair
+    assert totals["attn_kv4_decode"][2:] == [230 * 2 * 144 // 2 * 1.0 + 2 * 2 * 8 * 64 * 2, 4.0 * 8 * 64 * 230]
+    assert all(v[0] == 1 and v[1] > 0 and v[2] > 0 for v in totals.values())
