@@ -302,8 +302,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // is summed in 32 bits.
 // What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 404 of them, 288 of which are
 // its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products); four warps
-// a scheduler issue on 61 % of the cycles, the logical pipe is busy for half of them, and the memory gives 3.2 TB/s of 6.45
-// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 53.6 us, 26.7 at the memory's rate).  Three blocks an SM with
+// a scheduler issue on 62 % of the cycles, the logical pipe is busy for half of them, and the memory gives 3.2 TB/s of 6.45
+// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 50.9 us, 26.7 at the memory's rate).  Three blocks an SM with
 // 168 registers and no spills are no faster.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -721,52 +721,87 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
   }
 }
 
-// out[row] from the partial results of its splits, in their order; one block a (row, head).  Rows of one split are
-// finished already.
-template <typename T>
-__global__ void kv4_merge_kernel(const Kv4AttnArgs a, int D, int per_group) {
-  const size_t row = blockIdx.x, p0 = row * a.n_splits;
-  const int d = threadIdx.x, G = a.nq / a.nkv, hgroups = (G + per_group - 1) / per_group, h = row % a.nq;
-  const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
+// out[row] from the partial results of its splits, in their order; a warp a (row, head): its lanes take the splits'
+// factors first, a split a lane, and then D / 32 elements each through all splits.  Rows of one split are finished
+// already.  (With a thread for every element, which took the factors for itself, 60 sequences of up to 4,096 keys took
+// 53.6 us with their merging, now 50.9, and two of 32,768 29.9, now 27.8.)
+#define MERGE_WARPS 4
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4AttnArgs a, int per_group) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31, G = a.nq / a.nkv, hgroups = (G + per_group - 1) / per_group;
+  const long long row = (long long)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
   pdl_wait();                                        // (every block: the next kernel waits for this one only)
-  const int n = a.pieces[row / a.nq * a.nkv * hgroups + h / G * hgroups + h % G / per_group];
+  if (row >= (long long)a.n_rows * a.nq) return;
+  const int t = (int)(row / a.nq), h = (int)(row % a.nq);
+  const int n = a.pieces[(size_t)t * a.nkv * hgroups + h / G * hgroups + h % G / per_group];
   if (n <= 1) return;
+  float x[E];
+  float M, L;
   if (n > a.n_splits) {                               // keys beyond the caller's bound: some were left out
-    reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(__int_as_float(0x7fffffff));
-    if (a.lse && d == 0) a.lse[row] = __int_as_float(0x7fffffff);
-    return;
-  }
-  // (loads are requested eight splits at a time and used in split order)
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
-  float M = sk, L = 0.f, O = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 8) {
-    float2 v[8];
+    M = L = __int_as_float(0x7fffffff);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = ml[min(s0 + u, n - 1)];
+    for (int e = 0; e < E; ++e) x[e] = L;
+  } else {
+    const size_t p0 = (size_t)row * a.n_splits;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
+    const float* po = a.part_o + p0 * D + lane * E;
+    const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
+    float2 mine = make_float2(-INFINITY, 0.f);        // of split `lane` of the first 32 (of 32 at a time, below)
+    if (lane < n) mine = ml[lane];
+    M = mine.x;
+    for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
+    M = fmaxf(warp_max(M), sk);
+    L = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) M = fmaxf(M, v[u].x);
-  }
-  if (sk != -INFINITY) L = exp2f(sk - M);
-  for (int s0 = 0; s0 < n; s0 += 8) {
-    float2 v[8];
-    float o[8];
+    for (int e = 0; e < E; ++e) x[e] = 0.f;
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      if (s0 > 0) mine = s0 + lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+      const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - M);
+      L += mine.x == -INFINITY ? 0.f : mine.y * f;
+      const int here = min(32, n - s0);
+      // (eight splits' loads on their way at a time; those behind the last have the factor 0)
+      for (int s = 0; s < here; s += 8) {
+        float v[8][E];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int s = min(s0 + u, n - 1);
-      v[u] = ml[s];
-      o[u] = a.part_o[(p0 + s) * D + d];
-    }
+        for (int u = 0; u < 8; ++u) {
+          const float* from = po + (size_t)(s0 + min(s + u, here - 1)) * D;
+          if constexpr (E == 4) {
+            const float4 w = *reinterpret_cast<const float4*>(from);
+            v[u][0] = w.x, v[u][1] = w.y, v[u][2] = w.z, v[u][3] = w.w;
+          } else {
+            const float2 w = *reinterpret_cast<const float2*>(from);
+            v[u][0] = w.x, v[u][1] = w.y;
+          }
+        }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (s0 + u < n && v[u].x != -INFINITY) {
-        const float f = exp2f(v[u].x - M);
-        L += v[u].y * f;
-        O += o[u] * f;
+        for (int u = 0; u < 8; ++u) {
+          const float fs = __shfl_sync(0xffffffffu, f, min(s + u, 31));
+          // (a split that saw nothing has no sums)
+          if (s + u < here && fs != 0.f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = fmaf(v[u][e], fs, x[e]);
+          }
+        }
       }
     }
+    L = warp_sum(L);
+    if (sk != -INFINITY) L += exp2f(sk - M);
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] *= inv;
   }
-  reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(L != 0.f ? O / L : 0.f);
-  if (a.lse && d == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+  T* to = reinterpret_cast<T*>(a.out) + (size_t)row * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) to[e] = from_f32<T>(x[e]);
+  if (a.lse && lane == 0) a.lse[row] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T>
+static int merge(const Kv4AttnArgs& a, int D, int per_group, cudaStream_t s) {
+  const long long blocks = ((long long)a.n_rows * a.nq + MERGE_WARPS - 1) / MERGE_WARPS;
+  if (D == 64) return gb_launch(kv4_merge_kernel<T, 64>, dim3((unsigned)blocks), dim3(32 * MERGE_WARPS), 0, s, a, per_group);
+  return gb_launch(kv4_merge_kernel<T, 128>, dim3((unsigned)blocks), dim3(32 * MERGE_WARPS), 0, s, a, per_group);
 }
 
 // ---------------------------------------------------------------- 32 bits
@@ -1115,7 +1150,7 @@ static int decode(const Kv4AttnArgs& a, int blocks, cudaStream_t s) {
   const unsigned grid = (unsigned)(a.shared == 1 ? blocks : pairs * a.n_splits);
   const int rc = a.window > 0 || a.chunk > 0 ? decode_launch<D, true>(a, grid, s) : decode_launch<D, false>(a, grid, s);
   if (rc || a.n_splits == 1 || a.shared == 2) return rc;
-  return gb_launch(kv4_merge_kernel<bf16>, dim3((unsigned)(a.n_rows * a.nq)), dim3(D), 0, s, a, D, 8);
+  return merge<bf16>(a, D, 8, s);
 }
 
 // `blocks`: how many share the keys out (a->shared 1).
@@ -1143,7 +1178,7 @@ GB_EXPORT int gb_attn_kv4_f32(const Kv4AttnArgs* a, int D, cudaStream_t s) {
   rc = D == 64 ? gb_launch_cluster(kv4_f32_kernel<64>, grid, dim3(KV4_F32_WARPS * 32), 0, s, cluster, *a)
                : gb_launch_cluster(kv4_f32_kernel<128>, grid, dim3(KV4_F32_WARPS * 32), 0, s, cluster, *a);
   if (rc || a->n_splits == 1 || cluster > 1) return rc;
-  return gb_launch(kv4_merge_kernel<float>, dim3((unsigned)(a->n_rows * a->nq)), dim3(D), 0, s, *a, D, KV4_F32_HEADS);
+  return merge<float>(*a, D, KV4_F32_HEADS, s);
 }
 
 // `blocks`: blocks along the keys of every (kv head, sequence).

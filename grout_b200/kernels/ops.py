@@ -1929,7 +1929,7 @@ def kv4_read(pages: torch.Tensor, *, token_seq, token_pos, slots, block_table, p
 
 KV4_PER_SM = 4             # blocks of the bfloat16 kernel that an SM holds
 KV4_LEAST = 8              # stretches of 32 keys that a block takes at least (two for each of its warps)
-KV4_MOST = 16, 64          # up to so many a block may have of its own: a split's, a whole pair's
+KV4_MOST = 8, 16, 48       # up to so many a block may have of its own: one of many splits, one of up to four, a whole pair's
 KV4_SPLIT_OVERRIDE: Optional[int] = None      # stretches that a block takes at least, for experiments
 KV4_SHARE_OVERRIDE: Optional[int] = None      # how pairs are split (0, 1 or 2, see kv4_split_plan), for tests
 
@@ -1940,17 +1940,17 @@ def kv4_split_plan(n_seqs: int, pairs: int, keys: int, max_pages: int, sms: int)
     merge); 2: the splits of a pair are a cluster of up to eight blocks that merges them; 1: four blocks an SM share all
     stretches out, at least so many each, and a pair has at most so many splits.
 
-    Sharing out and merging cost some 6 us, which the even shares must be worth.  Measured, us, 32 heads of 128 on 8,
+    Sharing out and merging cost some 5 us, which the even shares must be worth.  Measured, us, 32 heads of 128 on 8,
     sequences of a sixth of the given lengths up to them, shared out (or merged) / a block a pair or a cluster: 64 of 300
-    17.9 / 10.2, of 1,024 25.6 / 20.7, of 1,500 29.7 / 26.6, of 2,048 35.7 / 36.0, of 3,000 44.9 / 48.0; 200 of 1,200
-    64.1 / 55.1; clusters: 32 of 1,000 18.3 / 15.6, one of 1,100 8.6 / 8.0, of 4,096 9.4 / 9.9, eight of 8,192 20.1 /
-    24.7, sixteen of 4,096 21.5 / 23.8."""
+    16.5 / 10.2, of 1,024 23.3 / 20.7, of 1,500 27.3 / 26.7, of 2,048 33.4 / 36.0, of 3,000 42.5 / 48.0; 200 of 1,200
+    59.1 / 55.5; clusters of two: 32 of 1,000 17.5 / 15.6; of four: 16 of 4,096 21.0 / 23.9; of up to eight: one of 300 8.2 /
+    7.0, of 1,100 8.6 / 8.0, of 4,096 8.8 / 9.9, eight of 2,100 12.5 / 13.9, of 8,192 19.5 / 24.7."""
     tiles, blocks = max(1, (keys + 31) // 32), KV4_PER_SM * sms
     least, way = KV4_SPLIT_OVERRIDE, KV4_SHARE_OVERRIDE
     if way is None:
         own = max(KV4_LEAST, -(-tiles // max(1, min(8, blocks // pairs))))
         splits = -(-tiles // own)
-        if own <= KV4_MOST[splits == 1] and not least:
+        if own <= KV4_MOST[2 if splits == 1 else splits <= 4] and not least:
             return (splits, own, 2) if splits > 1 else (1, tiles, 0)
     least = least or max(KV4_LEAST, -(-tiles // 62))
     splits = -(-tiles // least)
