@@ -926,13 +926,12 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       if (!any) continue;                                  // (not seen, or of no weight: whatever its pair holds)
       const uint32_t pr = reinterpret_cast<const uint32_t*>(rec + F::PAIR_OFF + tok * F::PAIR)[NG + group];
       const uint32_t w = reinterpret_cast<const uint32_t*>(rec + F::V_OFF + tok * F::ROW)[F::value_word(word, tok)];
-      const float sc = kv4_s(pr), mn = kv4_m(pr);
+      float x[8];
+      kv4_values(w, pr, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = fmaf(sc, (float)kv4_code(w, e), mn);
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-        for (int h = 0; h < HC; ++h) o[h][e] = fmaf(p[h], x, o[h][e]);
-      }
+        for (int h = 0; h < HC; ++h) o[h][e] = fmaf(p[h], x[e], o[h][e]);
     }
   }
   pdl_launch_dependents();

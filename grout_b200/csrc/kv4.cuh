@@ -56,11 +56,17 @@ __device__ __forceinline__ int kv4_page(const int* table, int tile, int max_page
 __device__ __forceinline__ float kv4_s(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float kv4_m(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// Two codes of a word (nibbles i and 4 + i) as the bfloat16 numbers 1 + c / 16: the code is the top of the mantissa.
-template <int I>
-__device__ __forceinline__ uint32_t kv4_two(uint32_t w) {
-  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (x & 0x00780078u) | 0x3f803f80u;
+// Code of element E (0..7) of a word, as a float: the low bits of 2^23's mantissa, less 2^23 (a conversion of whole
+// numbers has a quarter of the rate).
+template <int E>
+__device__ __forceinline__ float kv4_code(uint32_t w) {
+  constexpr int AT = ((E & 1) << 4) + ((E >> 1) << 2);
+  return __uint_as_float(((w >> AT) & 15u) | 0x4b000000u) - 8388608.f;
 }
-// Code of element e (0..7) of a word.
-__device__ __forceinline__ int kv4_code(uint32_t w, int e) { return (w >> (((e & 1) << 4) + ((e >> 1) << 2))) & 15; }
+// The eight elements of a word.
+__device__ __forceinline__ void kv4_values(uint32_t w, uint32_t pair, float (&x)[8]) {
+  const float s = kv4_s(pair), m = kv4_m(pair);
+  x[0] = fmaf(s, kv4_code<0>(w), m), x[1] = fmaf(s, kv4_code<1>(w), m), x[2] = fmaf(s, kv4_code<2>(w), m);
+  x[3] = fmaf(s, kv4_code<3>(w), m), x[4] = fmaf(s, kv4_code<4>(w), m), x[5] = fmaf(s, kv4_code<5>(w), m);
+  x[6] = fmaf(s, kv4_code<6>(w), m), x[7] = fmaf(s, kv4_code<7>(w), m);
+}

@@ -169,10 +169,8 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) kv4_read_kernel(const Kv4Rows
 #pragma unroll
     for (int u = 0; u < ROWS_AT_ONCE; ++u) {
       if (i0 + 32 * u >= words) break;
-      const float s = kv4_s(pair[u]), m = kv4_m(pair[u]);
       float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)kv4_code(w[u], e), m);
+      kv4_values(w[u], pair[u], x);
       store8(out + (size_t)(i0 + 32 * u) * 8, x);
     }
   }
