@@ -300,10 +300,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // below 2^8, so it stays below 2^15 and what it loses at the other end is below 2^-25 of a whole probability.  Values
 // are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range; m + 8 s times P
 // is summed in 32 bits.
-// What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 404 of them, 288 of which are
+// What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 403 of them, 288 of which are
 // its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products); four warps
-// a scheduler issue on 62 % of the cycles, the logical pipe is busy for half of them, and the memory gives 3.2 TB/s of 6.45
-// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 50.9 us, 26.7 at the memory's rate).  Three blocks an SM with
+// a scheduler issue on 62 % of the cycles, the logical pipe is busy for 47 %, and the memory gives 3.2 TB/s of 6.45
+// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 50.6 us, 26.7 at the memory's rate).  Three blocks an SM with
 // 168 registers and no spills are no faster.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsArgs a) {
 
 // The other way: a word and its pair in, eight elements out (zeros for a token that is nowhere).  A warp has a token,
 // finds once where it lives and has ROWS_AT_ONCE turns' loads on their way together.  (A thread for every word, which
-// found the token for itself by four loads in a row, read 16,384 tokens of 8 heads of 128 in 29.3 us, this in 16.0: 86 MB
-// at 5.4 TB/s.)
+// found the token for itself by four loads in a row, read 16,384 tokens of 8 heads of 128 in 29.3 us, this in 16.8: 86 MB
+// at 5.1 TB/s.)
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * ROWS_WARPS) kv4_read_kernel(const Kv4RowsArgs a) {
   using F = Kv4<D>;
