@@ -757,8 +757,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
     for (int e = 0; e < E; ++e) x[e] = 0.f;
     for (int s0 = 0; s0 < n; s0 += 32) {
       if (s0 > 0) mine = s0 + lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+      // (a maximum drops NaN, so a split that saw nothing but NaN has the factor 0 and a sum that is NaN: it has to stay)
       const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - M);
-      L += mine.x == -INFINITY ? 0.f : mine.y * f;
+      L += mine.y * f;
       const int here = min(32, n - s0);
       // (eight splits' loads on their way at a time; those behind the last have the factor 0)
       for (int s = 0; s < here; s += 8) {
