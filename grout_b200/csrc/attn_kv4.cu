@@ -778,10 +778,10 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           const float fs = __shfl_sync(0xffffffffu, f, min(s + u, 31));
-          // (a split that saw nothing has no sums)
-          if (s + u < here && fs != 0.f) {
+          if (s + u < here) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = fmaf(v[u][e], fs, x[e]);
+            for (int e = 0; e < E; ++e)                // (of a split without weight only what is NaN: an infinite sum is not)
+              if (fs != 0.f || v[u][e] != v[u][e]) x[e] = fmaf(v[u][e], fs, x[e]);
           }
         }
       }
@@ -917,14 +917,10 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
     for (int j = half; j < n_keys; j += KEYS) {
       const int tok = j % KV4_TOKENS;
       const uint8_t* rec = base + (j / KV4_TOKENS) * F::RECORD;
+      if (key0 + j < list.lo && key0 + j >= keep) continue;     // (not seen: whatever its pair holds)
       float p[HC];
-      bool any = false;
 #pragma unroll
-      for (int h = 0; h < HC; ++h) {
-        p[h] = p_s[warp][j][h];
-        any = any || p[h] != 0.f;
-      }
-      if (!any) continue;                                  // (not seen, or of no weight: whatever its pair holds)
+      for (int h = 0; h < HC; ++h) p[h] = p_s[warp][j][h];
       const uint32_t pr = reinterpret_cast<const uint32_t*>(rec + F::PAIR_OFF + tok * F::PAIR)[NG + group];
       const uint32_t w = reinterpret_cast<const uint32_t*>(rec + F::V_OFF + tok * F::ROW)[F::value_word(word, tok)];
       float x[8];

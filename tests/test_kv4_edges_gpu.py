@@ -45,3 +45,20 @@ def test_keys_that_are_nan(n, first, last, dtype, stretches, way, monkeypatch):
     out, lse = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=step, page=64, scale=0.1, want_lse=True)
     assert bool(out[0, :4].isnan().all()) and bool(lse[0, :4].isnan().all())
     assert not bool(out[0, 4:].isnan().any()) and not bool(out[1].isnan().any()) and not bool(lse[0, 4:].isnan().any())
+
+
+@pytest.mark.parametrize("dtype,stretches,way", SPLITS)
+@pytest.mark.parametrize("n,first,last", [(700, 0, 256), (700, 699, 700), (257, 3, 4)])
+def test_values_that_are_nan_and_of_no_weight(n, first, last, dtype, stretches, way, monkeypatch):
+    """A token that a row sees makes its 64 elements NaN when they are stored as NaN, though 2^(its score) is 0."""
+    split(monkeypatch, stretches, way)
+
+    def edit(kv):
+        kv[first:last, :2, 3] = -900.0
+        kv[first:last, 3, :64] = NAN                              # the values of kv head 1
+    c = Cache([n, 90], 2, 128, dtype, seed=1, edit=edit)
+    step, q = c.step([1, 1]), queries(2, 8, 128, dtype, 0)
+    q[..., 3] = 4.0
+    out = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=step, page=64, scale=0.1)
+    assert bool(out[0, 4:, :64].isnan().all())
+    assert not bool(out[0, :4].isnan().any()) and not bool(out[0, 4:, 64:].isnan().any()) and not bool(out[1].isnan().any())
