@@ -549,13 +549,14 @@ attn_prefill_tc_kernel(const __grid_constant__ typename Source::Params source, c
       // raise the base only when the maximum outgrew it by 2^8 (or on the first keys)
       float factor = 1.0f;
       const bool raise = mx > m_used + 8.0f;       // also true when m_used is -inf and mx is finite
+      const bool held = raise && m_used != -INFINITY;   // (a factor that has become 0 counts: the old sums go)
       if (raise) {
         factor = (m_used == -INFINITY) ? 0.f : fast_exp2(m_used - mx);
         m_used = mx;
       }
       // rows of O that already hold products must be rescaled; the load and store of
       // tensor memory are warp-wide, so the warp does it when any lane has to
-      const bool rescale = __any_sync(0xffffffffu, raise && j > 0 && factor != 0.f);
+      const bool rescale = __any_sync(0xffffffffu, held);
       if (rescale) {
         // S_j is complete, so the product of tile j-2, issued before it, is too:
         // o_done is at most one phase behind

@@ -1,9 +1,12 @@
 """Where the operators on a 4-bit cache could go wrong: at the edges of what they are given."""
+import math
+
 import pytest
 import torch
 
 from grout_b200.kernels import ops
-from test_kv4_gpu import DEV, NAN, Cache, queries
+from plain import kv4
+from test_kv4_gpu import DEV, NAN, Cache, check, queries
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -62,3 +65,56 @@ def test_values_that_are_nan_and_of_no_weight(n, first, last, dtype, stretches, 
     out = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=step, page=64, scale=0.1)
     assert bool(out[0, 4:, :64].isnan().all())
     assert not bool(out[0, :4].isnan().any()) and not bool(out[0, 4:, 64:].isnan().any()) and not bool(out[1].isnan().any())
+
+
+# ---------------------------------------------------------------- scores far apart
+def far_apart(nq, D, rows):
+    """Keys whose scores lie 400 and more below those of the later ones (natural units), and queries of the last rows."""
+    def edit(kv):
+        nkv = kv.shape[1] // 2
+        kv[:, :nkv, 3] = 0.0
+        kv[:130, :nkv, 3] = -50.0
+        kv[130:, :nkv, 3] = 50.0
+        kv[:130, nkv:] += 6.0                                      # values that would be seen in the result
+    c = Cache([260], 2, D, BF16, seed=3, edit=edit)
+    q = queries(rows, nq, D, BF16, 5)
+    q[..., 3] = 32.0
+    return c, q
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [0, 128, 256])
+def test_a_maximum_that_rises_beyond_the_numbers_range(rows, D, monkeypatch):
+    """2^(old maximum - new) is 0 in 32 bits: nothing of the earlier keys is left, in a prompt's rows and a single token's."""
+    monkeypatch.setattr(ops, "PREFILL_TC_ROWS", rows)
+    c, q = far_apart(8, D, 260)
+    scale = 1.0 / math.sqrt(D)
+    for n in (260, 1):
+        step = c.step([n])
+        out, lse = ops.attention_kv4(q[260 - n:].to(DEV), c.pages, c.table, step=step, page=64, scale=scale, want_lse=True)
+        check(out.cpu(), lse.cpu(), c, 0, q[260 - n:], n, scale, BF16, n > 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [128, 256])
+def test_a_maximum_that_rises_beyond_the_range_over_pages_in_16_bits(rows, D):
+    c, q = far_apart(8, D, 260)
+    step, scale = c.step([260]), 1.0 / math.sqrt(D)
+    rows_of = torch.arange(260)
+    k, v = c.kv[:, :2].bfloat16(), c.kv[:, 2:].bfloat16()
+    k_pages, v_pages = (torch.zeros((c.pages.shape[0], 2, 64, D), dtype=BF16, device=DEV) for _ in range(2))
+    table = c.table.cpu()
+    for p in range(5):
+        at = rows_of[64 * p:64 * p + 64]
+        k_pages[int(table[c.slots[0], p]), :, :len(at)] = k[at].transpose(0, 1).to(DEV)
+        v_pages[int(table[c.slots[0], p]), :, :len(at)] = v[at].transpose(0, 1).to(DEV)
+    out = ops.attn_prefill_tc(q.to(DEV), k_pages, v_pages, c.table, cu_q=step.cu_q, slots=step.slots, kv_len=step.kv_len,
+                              q_lens=step.q_lens, page=64, scale=scale, rows_per_block=rows).cpu()
+    want, _l, p = kv4.attend(q, k.transpose(0, 1), v.transpose(0, 1), scale)
+    for h in range(8):
+        av = v[:, h // 4].double().abs()
+        # the output's rounding, the probabilities' (2^-8 each), and 2^-17 of scores up to 400 + 128 * 16
+        delta = 2.0 ** -17 * 400
+        tol = (2.0 ** -8 + 2 * delta) * want[:, h].abs() + (2.0 ** -8 * (1 + 2.0 ** -7) + 2 * delta) * (p[h] @ av)
+        off = (out[:, h].double() - want[:, h]).abs()
+        assert bool((off <= tol).all()), (h, float((off / tol).max()))
