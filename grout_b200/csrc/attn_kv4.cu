@@ -778,11 +778,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           const float fs = __shfl_sync(0xffffffffu, f, min(s + u, 31));
-          if (s + u < here) {
+          // (also where the factor is 0: a sum that is NaN has to stay)
 #pragma unroll
-            for (int e = 0; e < E; ++e)                // (of a split without weight only what is NaN: an infinite sum is not)
-              if (fs != 0.f || v[u][e] != v[u][e]) x[e] = fmaf(v[u][e], fs, x[e]);
-          }
+          for (int e = 0; e < E; ++e) x[e] = fmaf(v[u][e], fs, x[e]);
         }
       }
     }
