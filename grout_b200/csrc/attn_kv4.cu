@@ -144,6 +144,12 @@ struct Kv4Decode {
   static constexpr int SMEM = RING + MERGE + 128;
 };
 
+// The least score there is (minus infinity would make a NaN of a difference), and the largest power of two that P s is
+// multiplied by: P of up to 2^8 times it is a number.
+#define KV4_NO_BASE -3e38f
+#define KV4_DOWN_MOST 118
+__device__ __forceinline__ float kv4_power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e
+
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
@@ -295,11 +301,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 //   P = 2^(S c - m) in registers; times the value's s it becomes the B operand of the second product by a transposition
 //                   of 8 x 8 numbers among the lanes
 //   O += V^T P      rows the head's elements, columns heads
-// so the codes go from shared memory straight into operands.  P s is half-precision: it is divided by a power of two
-// near the largest s that the warp has met (raised when an s is 2^6 beyond it), and the base of the exponents keeps P
-// below 2^8, so it stays below 2^15 and what it loses at the other end is below 2^-25 of a whole probability.  Values
-// are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range; m + 8 s times P
-// is summed in 32 bits.
+// so the codes go from shared memory straight into operands.  P s is half-precision, in units of a power of two for each
+// head and group of 64 elements: the largest P s that there was when the unit was chosen, by which a value's s may then be
+// exceeded 2^6 times before it is chosen again.  The base of the exponents keeps P below 2^8, so P s stays below 2^15 units,
+// and what it loses at the other end is below 2^-25 of one.  (Units by the largest s alone, whatever its token was paid, were
+// 1 us faster on the case below, 4 % with many short sequences, and lost all of the others' values beside one 10^9 times as
+// large.)  Values are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range;
+// m + 8 s times P is summed in 32 bits.
 // What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 403 of them, 288 of which are
 // its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products); four warps
 // a scheduler issue on 62 % of the cycles, the logical pipe is busy for 47 %, and the memory gives 3.2 TB/s of 6.45
@@ -495,14 +503,17 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
     const float unit_scale = capped ? a.cap.cap_inv : a.scale_log2;
     const float factor[2] = {unit_scale * q.back[0], unit_scale * q.back[1]};
 
-    // of heads 2 t, 2 t + 1: the base of the exponents, the base or 0 where there is none, the base and 2^8; the sum of
-    // P and of P (m + 8 s) over this lane's rows
-    float m[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f}, most[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // of heads 2 t, 2 t + 1: the base of the exponents (a whole number; KV4_NO_BASE: none yet); the sum of P and of P (m + 8 s)
+    // over this lane's rows
+    float base[2] = {KV4_NO_BASE, KV4_NO_BASE}, l[2] = {0.f, 0.f};
     float o[NG][4][4], off[NG][2];
-    float s_most = 0.f, s_down = 1.f;                // an s beyond the first raises the power of two; its inverse
+    // of a group: the powers of two that P s is multiplied by, and the s beyond which they are looked at again
+    float down[NG][2], s_most[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       off[g][0] = off[g][1] = 0.f;
+      down[g][0] = down[g][1] = kv4_power(KV4_DOWN_MOST);
+      s_most[g] = kv4_power(6 - KV4_DOWN_MOST);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -559,43 +570,64 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
               }
             }
         }
-        // the base of a head's exponents is raised only when a score has outgrown it by 2^8 (or is the first)
-        float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]), sv = 0.f;
+        // The base of a head's exponents is raised only when a score has outgrown it by 2^8 (or is the first), by a whole
+        // number, and the unit of P s, 1 / down, is looked at again then and when an s is beyond those met so far: it becomes
+        // the largest P s that there was or is, so that neither a large value without weight nor one that lost its weight
+        // takes bits from the others.
+        float x[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
 #pragma unroll
-        for (int u = 1; u < NR; ++u) x0 = fmaxf(x0, fmaxf(s[u][0], s[u][2])), x1 = fmaxf(x1, fmaxf(s[u][1], s[u][3]));
+        for (int u = 1; u < NR; ++u) x[0] = fmaxf(x[0], fmaxf(s[u][0], s[u][2])), x[1] = fmaxf(x[1], fmaxf(s[u][1], s[u][3]));
+        bool outgrown = x[0] > base[0] + 8.f || x[1] > base[1] + 8.f;
 #pragma unroll
-        for (int u = 0; u < NR; ++u)
+        for (int g = 0; g < NG; ++g) {
+          float sv = 0.f;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) sv = fmaxf(sv, fmaxf(kv4_s(vp[u][0][g]), kv4_s(vp[u][1][g])));
-        if (__any_sync(0xffffffffu, x0 > most[0] || x1 > most[1] || sv > s_most)) {
+          for (int u = 0; u < NR; ++u) sv = fmaxf(sv, fmaxf(kv4_s(vp[u][0][g]), kv4_s(vp[u][1][g])));
+          outgrown = outgrown || sv > s_most[g];
+        }
+        if (__any_sync(0xffffffffu, outgrown)) {
+          float f[2];
+          int steps[2];
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-            sv = fmaxf(sv, __shfl_xor_sync(0xffffffffu, sv, d));
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], d));
+            const float to = fmaxf(base[i], ceilf(x[i])), by = fminf(to - base[i], 1000.f);
+            f[i] = exp2_fast(-by), steps[i] = (int)by;
+            l[i] *= f[i];
+            base[i] = to;
           }
-          float down = s_down;
-          if (sv > s_most) {                         // (the same in all lanes: a row's pairs are its four lanes')
-            const int e = min(max((int)(__float_as_uint(sv) >> 23), 1), 247);
-            down = __uint_as_float((uint32_t)(254 - e) << 23);
-            s_most = __uint_as_float((uint32_t)(e + 6) << 23);
-          }
-          const float change = down / s_down;
-          s_down = down;
-          x0 = fmaxf(x0, m[0]), x1 = fmaxf(x1, m[1]);
-          const float f0 = m[0] == -INFINITY ? 0.f : exp2_fast(m[0] - x0);
-          const float f1 = m[1] == -INFINITY ? 0.f : exp2_fast(m[1] - x1);
-          m[0] = x0, m[1] = x1;
-          base[0] = x0 == -INFINITY ? 0.f : x0, base[1] = x1 == -INFINITY ? 0.f : x1;
-          most[0] = x0 + 8.f, most[1] = x1 + 8.f;
-          l[0] *= f0, l[1] *= f1;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            off[g][0] *= f0, off[g][1] *= f1;
+            float w[2] = {0.f, 0.f};                 // (a NaN has no part)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int u = 0; u < NR; ++u)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[g][i][c] *= ((c & 1) ? f1 : f0) * change;
+              for (int c = 0; c < 4; ++c)
+                w[c & 1] = fmaxf(w[c & 1], exp2_fast(s[u][c] - base[c & 1]) * kv4_s(vp[u][c >> 1][g]));
+            // the exponents of both heads' in one word
+            uint32_t both = __byte_perm(__float_as_uint(w[0]), __float_as_uint(w[1]), 0x7632);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+            int most = -KV4_DOWN_MOST;
+            float change[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              // (the old sums' unit, and the new one: the exponents of their inverses)
+              const int was = (int)(__float_as_uint(down[g][i]) >> 23) - 127 + steps[i];
+              const int now = min(min(was, KV4_DOWN_MOST), max(127 - (int)(i ? both >> 23 : both >> 7 & 255), -KV4_DOWN_MOST));
+              change[i] = kv4_power(max(now - was, -126));
+              down[g][i] = kv4_power(now);
+              most = max(most, now);
+              off[g][i] *= f[i];
+            }
+            s_most[g] = kv4_power(6 - most);
+            if (k > 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[g][i][c] *= change[c & 1];
+            }
           }
         }
 #pragma unroll
@@ -617,9 +649,9 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
             const float ma = fmaf(8.f, sa, kv4_m(vp[u][0][g])), mb = fmaf(8.f, sb, kv4_m(vp[u][1][g]));
             off[g][0] = fmaf(p[2], mb, fmaf(p[0], ma, off[g][0]));
             off[g][1] = fmaf(p[3], mb, fmaf(p[1], ma, off[g][1]));
-            const float ra = sa * s_down, rb = sb * s_down;
-            const uint32_t p0 = transposed8x8(as_u32(__floats2half2_rn(p[0] * ra, p[1] * ra)));
-            const uint32_t p1 = transposed8x8(as_u32(__floats2half2_rn(p[2] * rb, p[3] * rb)));
+            const float d0 = down[g][0], d1 = down[g][1];
+            const uint32_t p0 = transposed8x8(as_u32(__floats2half2_rn(p[0] * d0 * sa, p[1] * d1 * sa)));
+            const uint32_t p1 = transposed8x8(as_u32(__floats2half2_rn(p[2] * d0 * sb, p[3] * d1 * sb)));
             uint32_t ya[4], za[4], yb[4], zb[4];
             kv4_codes(__byte_perm(va[0][g], va[1][g], 0x5410), magic, ya);
             kv4_codes(__byte_perm(va[0][g], va[1][g], 0x7632), magic, za);
@@ -637,7 +669,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
         ask(next, turn + C::STAGES);
       }
     }
-    if (__any_sync(0xffffffffu, lost)) m[0] = m[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
+    if (__any_sync(0xffffffffu, lost)) base[0] = base[1] = 0.f, l[0] = l[1] = __int_as_float(0x7fffffff);
 
     const bool again = more;
     turn_of ^= 1;
@@ -655,8 +687,12 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
         off[g][1] += __shfl_xor_sync(0xffffffffu, off[g][1], d);
       }
     }
+    float up[NG][2];                                   // 1 / down
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) up[g][i] = __uint_as_float((254u << 23) - __float_as_uint(down[g][i]));
     __syncthreads();                                   // every warp has read the results of the part before
-    const float s_up = 1.f / s_down;                   // (a power of two)
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -664,11 +700,11 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           red_o[(warp * 8 + 2 * t + (c & 1)) * C::PITCH + ((g * 4 + i) * 2 + (c >> 1)) * 8 + r] =
-              fmaf(s_up, o[g][i][c], off[g][c & 1]);
+              fmaf(up[g][c & 1], o[g][i][c], off[g][c & 1]);
     if (r == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        red_ml[(warp * 8 + 2 * t + i) * 2] = m[i];
+        red_ml[(warp * 8 + 2 * t + i) * 2] = base[i] == KV4_NO_BASE ? -INFINITY : base[i];
         red_ml[(warp * 8 + 2 * t + i) * 2 + 1] = l[i];
       }
     }

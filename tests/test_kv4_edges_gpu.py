@@ -118,3 +118,54 @@ def test_a_maximum_that_rises_beyond_the_range_over_pages_in_16_bits(rows, D):
         tol = (2.0 ** -8 + 2 * delta) * want[:, h].abs() + (2.0 ** -8 * (1 + 2.0 ** -7) + 2 * delta) * (p[h] @ av)
         off = (out[:, h].double() - want[:, h]).abs()
         assert bool((off <= tol).all()), (h, float((off / tol).max()))
+
+
+# ---------------------------------------------------------------- values of very different sizes
+def sizes_apart(kind, nkv):
+    def edit(kv):
+        if kind == "a huge value that is paid nothing":
+            kv[5, :nkv, 3] = -600.0
+            kv[5, nkv:] *= 1e9
+        elif kind == "huge values that a later key outweighs":
+            kv[:200, :nkv, 3] = -600.0
+            kv[:200, nkv:] *= 1e9
+        elif kind == "huge values, then small ones that outweigh them":
+            kv[:200, :nkv, 3] = -600.0
+            kv[:200, nkv:] *= 1e20
+            kv[200:, nkv:] *= 1e-15
+        elif kind == "groups of different sizes":
+            kv[:, nkv:, :64] *= 1e7
+        elif kind == "small":
+            kv[:, nkv:] *= 1e-25
+        elif kind == "large":
+            kv[:, nkv:] *= 1e35
+        elif kind == "without a range":
+            kv[:, nkv:] = 0.75
+        elif kind == "growing":
+            kv[:, nkv:] *= torch.logspace(-12, 12, kv.shape[0])[:, None, None]
+        elif kind == "heads that pay to other tokens":
+            kv[::2, :nkv, 3], kv[1::2, :nkv, 3] = 600.0, -600.0
+            kv[::2, nkv:] *= 1e8
+    return edit
+
+
+KINDS = ["a huge value that is paid nothing", "huge values that a later key outweighs",
+         "huge values, then small ones that outweigh them", "groups of different sizes", "small", "large", "without a range",
+         "growing", "heads that pay to other tokens"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,stretches,way", [(BF16, None, None), (BF16, 2, 0), (BF16, 2, 1), (BF16, 2, 2), (F32, None, None)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_of_different_sizes(D, dtype, stretches, way, kind, monkeypatch):
+    """A value's steps may be any size: a probability times a step keeps its bits whatever the values beside it."""
+    split(monkeypatch, stretches, way)
+    c = Cache([330, 40], 2, D, dtype, seed=8, edit=sizes_apart(kind, 2))
+    q = queries(2, 16, D, dtype, 1)
+    q[..., 3] = 4.0
+    if kind == "heads that pay to other tokens":
+        q[:, ::2, 3] = -4.0
+    scale = 0.6 / math.sqrt(D)
+    out, lse = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=c.step([1, 1]), page=64, scale=scale, want_lse=True)
+    for i in range(2):
+        check(out[i:i + 1].cpu(), lse[i:i + 1].cpu(), c, i, q[i:i + 1], 1, scale, dtype, False)
