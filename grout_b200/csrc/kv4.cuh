@@ -8,7 +8,7 @@
 //
 // m is the group's smallest element rounded down to bfloat16 and s = (largest - m) / 15 rounded up, so that the range
 // [m, m + 15 s] holds the group, no code has to be cut off, and an element is off by at most s / 2.  A group whose
-// range bfloat16 cannot hold, or with an element that is not finite, is stored as NaN.
+// range bfloat16 cannot hold ([m, m + 15 s], not only its elements), or with an element that is not finite, is stored as NaN.
 //
 // The order of a row's 32-bit words is the order in which the threads of m16n8k16 products take them.  A word has
 // eight elements of the head, 8 n .. 8 n + 7 for word n: element 2 i in nibble i and 2 i + 1 in nibble 4 + i, so that

@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsArgs a) {
   const uint32_t sb = bf16_away(__fdiv_rn(__fsub_rn(hi, m), 15.f));               // upwards: it is not negative
   const float s = __uint_as_float(sb << 16);
   uint32_t word = 0, pair = (mb << 16) | sb;
-  if (!fine || !isfinite(s) || !isfinite(m)) {
+  // (the step is rounded up: m + 15 s may be no number where the largest element still is one)
+  if (!fine || !isfinite(s) || !isfinite(m) || !(fmaf(15.f, s, m) < 0x1.FFp127f)) {        // (half a step beyond bfloat16's last)
     pair = 0x7fff7fffu;                                         // NaN, NaN
   } else if (s > 0.f) {
     // (steps at the ends of the numbers' range are brought to its middle by a power of two, exactly)

@@ -6,7 +6,7 @@ import torch
 
 from grout_b200.kernels import ops
 from plain import kv4
-from test_kv4_gpu import DEV, NAN, Cache, check, queries
+from test_kv4_gpu import DEV, NAN, Cache, check, ints, queries
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -169,3 +169,21 @@ def test_values_of_different_sizes(D, dtype, stretches, way, kind, monkeypatch):
     out, lse = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=c.step([1, 1]), page=64, scale=scale, want_lse=True)
     for i in range(2):
         check(out[i:i + 1].cpu(), lse[i:i + 1].cpu(), c, i, q[i:i + 1], 1, scale, dtype, False)
+
+
+# ---------------------------------------------------------------- the end of the numbers' range
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_range_that_ends_beyond_the_numbers(dtype):
+    """Fifteen steps above the least element no finite number is left (the step is rounded up): such a group is NaN like
+    every other whose range is not held, and no row that does not see it has a part of it."""
+    def edit(kv):
+        kv[20, 1, :64] = 2e36
+        kv[20, 1, 7] = 3.3895e38                                   # (bfloat16's largest; a 15th of the range rounds up)
+        kv[21, 1, :64] = torch.linspace(0, 3.2e38, 64)             # held
+    c = Cache([100], 1, 64, dtype, edit=edit)
+    got = ops.kv4_read(c.pages, token_seq=ints(0, 0), token_pos=ints(20, 21), **c.at).cpu()
+    assert bool(got[0, 1].isnan().all()) and bool(got[1, 1].isfinite().all())
+    step, q = c.step([100]), queries(100, 4, 64, dtype, 1)
+    out = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=step, page=64, scale=0.125, window=10).cpu()
+    seen = out.isnan().any(-1).any(-1)
+    assert seen.nonzero().flatten().tolist() == list(range(20, 30))
