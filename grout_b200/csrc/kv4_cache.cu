@@ -381,7 +381,8 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
   const int slot = a.slots[seq];
   if ((unsigned)slot >= (unsigned)a.n_slots) return;
   const size_t head = (size_t)seq * a.nkv + h;
-  // lanes 0..15: where the record's tokens come from (as 16-token records and a place in them), -1: no such token
+  // lanes 0..15: where the record's tokens come from (as 16-token records and a place in them); -1: no such token, -2: one
+  // that no page holds, which goes on as NaN without a weight
   long long src = -1;
   if (lane < KV4_TOKENS) {
     const int j = rec * KV4_TOKENS + lane;
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
       if (a.in_order) from = j;
       if (a.from_table) {
         const int page = kv4_page(a.from_table + (size_t)slot * a.from_max, from / KV4_PAGE, a.from_max, a.n_pages);
-        if (page >= 0) src = ((long long)page * a.nkv + h) * KV4_PAGE + (from & (KV4_PAGE - 1));
+        src = page >= 0 ? ((long long)page * a.nkv + h) * KV4_PAGE + (from & (KV4_PAGE - 1)) : -2;
       } else {
         src = (long long)head * n_rec * KV4_TOKENS + from;
       }
@@ -412,6 +413,7 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
   for (int u = 0; u < KV4_TOKENS * KC / 32; ++u) {
     const int c = u * 32 + lane, tok = c / KC;
     const long long sp = __shfl_sync(0xffffffffu, src, tok);
+    k[u] = make_uint4(0, 0, 0, 0);
     if (sp >= 0)
       k[u] = *reinterpret_cast<const uint4*>(a.from + (size_t)(sp / KV4_TOKENS) * F::RECORD + (sp & 15) * F::ROW + (c % KC) * 16);
   }
@@ -420,6 +422,8 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
   for (int u = 0; u < KV4_TOKENS * VC / 32; ++u) {
     const int c = u * 32 + lane, tok = c / VC;
     const long long sp = __shfl_sync(0xffffffffu, src, tok);
+#pragma unroll
+    for (int g = 0; g < F::NG; ++g) v[u][g] = 0u;
     if (sp >= 0) {
       const int from_tok = sp & 15, chunk = (c % VC) ^ F::turn(tok) ^ F::turn(from_tok);
       const uint32_t* p = reinterpret_cast<const uint32_t*>(a.from + (size_t)(sp / KV4_TOKENS) * F::RECORD + F::V_OFF +
@@ -429,6 +433,8 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
     }
   }
   uint32_t pr[2 * F::NG];
+#pragma unroll
+  for (int g = 0; g < 2 * F::NG; ++g) pr[g] = 0x7fff7fffu;       // (NaN, NaN)
   float w = 0.f;
   if (src >= 0) {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(a.from + (size_t)(src / KV4_TOKENS) * F::RECORD + F::PAIR_OFF +
@@ -440,18 +446,18 @@ __global__ void __launch_bounds__(128) kv4_move_kernel(const Kv4MoveArgs a) {
 #pragma unroll
   for (int u = 0; u < KV4_TOKENS * KC / 32; ++u) {
     const int c = u * 32 + lane, tok = c / KC;
-    if (__shfl_sync(0xffffffffu, src, tok) >= 0) *reinterpret_cast<uint4*>(to + tok * F::ROW + (c % KC) * 16) = k[u];
+    if (__shfl_sync(0xffffffffu, src, tok) != -1) *reinterpret_cast<uint4*>(to + tok * F::ROW + (c % KC) * 16) = k[u];
   }
 #pragma unroll
   for (int u = 0; u < KV4_TOKENS * VC / 32; ++u) {
     const int c = u * 32 + lane, tok = c / VC;
-    if (__shfl_sync(0xffffffffu, src, tok) >= 0) {
+    if (__shfl_sync(0xffffffffu, src, tok) != -1) {
       uint32_t* p = reinterpret_cast<uint32_t*>(to + F::V_OFF + tok * F::ROW) + (c % VC) * F::NG;
 #pragma unroll
       for (int g = 0; g < F::NG; ++g) p[g] = v[u][g];
     }
   }
-  if (src >= 0) {
+  if (src != -1) {
     uint32_t* p = reinterpret_cast<uint32_t*>(to + F::PAIR_OFF + lane * F::PAIR);
 #pragma unroll
     for (int g = 0; g < 2 * F::NG; ++g) p[g] = pr[g];

@@ -2122,7 +2122,8 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     Returns (kept int32 [sequences, kv heads, keep]: the places that they stood at, -1 behind the last; the new lengths
     int32 [sequences]).  Sequences of slot -1 keep nothing, shorter ones all they have.  ``into``: a block table like
     ``block_table`` whose pages take the kept tokens (pages that no sequence of the call reads from); without it they
-    stay in the sequence's first pages.  A slot must not appear twice."""
+    stay in the sequence's first pages.  A token that no page holds is kept as NaN without a weight.  A slot must not
+    appear twice."""
     dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
     w = _take_weights(weights, n_pages, nkv, dev)
     table = _take(block_table, "block table", _I32, 2, dev)

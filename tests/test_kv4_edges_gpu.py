@@ -187,3 +187,34 @@ def test_a_range_that_ends_beyond_the_numbers(dtype):
     out = ops.attention_kv4(q.to(DEV), c.pages, c.table, step=step, page=64, scale=0.125, window=10).cpu()
     seen = out.isnan().any(-1).any(-1)
     assert seen.nonzero().flatten().tolist() == list(range(20, 30))
+
+
+# ---------------------------------------------------------------- eviction
+@pytest.mark.parametrize("place", ["in place", "elsewhere"])
+def test_eviction_of_tokens_that_no_page_holds(place):
+    """They are kept as NaN without a weight, whatever lay in the memory that they go to."""
+    n, keep, recent = 200, 100, 20
+    c = Cache([n], 2, 64, BF16, seed=4, weights=True, spare_pages=3)
+    good = torch.cat(c.sequence(0)).transpose(0, 1)
+    table = c.table.clone()
+    table[c.slots[0], 2], table[c.slots[0], 3] = -3, 1 << 30       # tokens 128 .. 191 and 192 .. 199
+    into = None
+    if place == "elsewhere":
+        into = torch.full((c.n_slots, 2), -1, dtype=torch.int32)
+        into[c.slots[0]] = torch.tensor(c.free[:2])
+        into = into.to(DEV)
+    kept, new = ops.kv4_evict(c.pages, c.weights, table, slots=ints(*c.slots), kv_len=ints(n), page=64, keep=keep, recent=recent,
+                              first=70, into=into)
+    assert new.tolist() == [keep]
+    to = table if into is None else into
+    got = ops.kv4_read(c.pages, token_seq=ints(*[0] * keep), token_pos=ints(*range(keep)), block_table=to, page=64,
+                       slots=ints(*c.slots)).cpu()
+    for h in range(2):
+        places = kept[0, h].tolist()
+        assert places[:70] == list(range(70)) and places[80:] == list(range(180, 200))
+        for j, p in enumerate(places):
+            w = float(c.weights[int(to[c.slots[0], j // 64]), h, j % 64])
+            if p >= 128:
+                assert bool(got[j, [h, 2 + h]].isnan().all()) and w == 0.0
+            else:
+                assert torch.equal(got[j, [h, 2 + h]], good[p, [h, 2 + h]])
