@@ -18,9 +18,9 @@ struct Kv4AttnArgs {
   const int* cu_q;         // [n_seqs + 1]
   void* out;               // [rows, nq, D]
   float* lse;              // [rows, nq] or null
-  float* part_o;           // [rows, nq, n_splits, D]   (n_splits > 1)
-  float* part_ml;          // [rows, nq, n_splits, 2]
-  int* pieces;             // [rows, nkv * groups of heads]: how many splits a row has (n_splits > 1)
+  float* part_o;           // [parts, heads of a group, D]   (n_splits > 1 and no clusters; see Kv4AttnArgs::part)
+  float* part_ml;          // [parts, heads of a group, 2]
+  int2* pieces;            // [rows, nkv * groups of heads]: how many parts a pair of row and group has, and its first
   int* error;
   const float* sinks;      // [nq] one more logit of every head's denominator, or null
   int n_rows, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window, n_splits;
@@ -29,6 +29,11 @@ struct Kv4AttnArgs {
   int keep_first, chunk;
   float scale_log2;
   ScoreCap cap;
+  // The first part of a pair whose first piece block `block` has.  Blocks that share the stretches out go through the pairs
+  // in their order, so that the sum of a block's number and a pair's is another one for every part, and there are no more
+  // parts than blocks and pairs: with a place for every split that the bound of the lengths allows, 64 sequences of up to
+  // 32,768 keys with 64 heads of 64 on 8 took 68 MB for what now has 2.3.
+  __device__ __forceinline__ int part(int pair, int block) const { return shared == 1 ? block + pair : pair * n_splits; }
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x, one instruction of the special unit; 2^-inf = 0
@@ -126,7 +131,7 @@ __device__ __forceinline__ void empty_row(const Kv4AttnArgs& a, int seq, int gro
   if (a.lse)
     for (int i = threadIdx.x; i < a.nq; i += blockDim.x)
       a.lse[(size_t)seq * a.nq + i] = live && a.sinks ? a.sinks[i] : -INFINITY;
-  for (int i = threadIdx.x; i < groups; i += blockDim.x) a.pieces[(size_t)seq * groups + i] = 1;
+  for (int i = threadIdx.x; i < groups; i += blockDim.x) a.pieces[(size_t)seq * groups + i] = make_int2(1, 0);
 }
 
 template <int D>
@@ -738,6 +743,8 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
       finish_cluster<bf16>(a, reinterpret_cast<const float*>(smem), red_h, done.seq, live, h0, heads, D, done.piece);
       break;
     }
+    const int pair = done.seq * groups + done.group, first = a.part(pair, blockIdx.x - done.piece);
+    const size_t row0 = (size_t)(first + done.piece) * min(8, G);
     for (int i = threadIdx.x; i < heads * D; i += C::WARPS * 32) {
       const int h = i / D, d = i % D, place = (d & 64) + (d & 7) * 8 + (d >> 3 & 7);
       float O = 0.f;
@@ -746,13 +753,12 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
       const float2 ml = red_h[h];
       if (alone) {
         finish_row<bf16>(a, done.seq, live, h0 + h, d, D, ml.x, ml.y, O);
-      } else if (done.piece < a.n_splits) {            // (more than the caller's bound of the lengths allows: merged as NaN)
-        const size_t row = (size_t)done.seq * a.nq + h0 + h;
-        a.part_o[(row * a.n_splits + done.piece) * D + d] = O;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.n_splits + done.piece) * 2) = ml;
+      } else {
+        a.part_o[(row0 + h) * D + d] = O;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row0 + h) * 2) = ml;
       }
     }
-    if (a.n_splits > 1 && done.piece == 0 && threadIdx.x == 0) a.pieces[done.seq * groups + done.group] = done.n_pieces;
+    if (a.n_splits > 1 && done.piece == 0 && threadIdx.x == 0) a.pieces[pair] = make_int2(done.n_pieces, first);
     if (!again) break;
   }
 }
@@ -770,7 +776,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
   pdl_wait();                                        // (every block: the next kernel waits for this one only)
   if (row >= (long long)a.n_rows * a.nq) return;
   const int t = (int)(row / a.nq), h = (int)(row % a.nq);
-  const int n = a.pieces[(size_t)t * a.nkv * hgroups + h / G * hgroups + h % G / per_group];
+  const int2 parts = a.pieces[(size_t)t * a.nkv * hgroups + h / G * hgroups + h % G / per_group];
+  const int n = parts.x, heads = min(per_group, G);
   if (n <= 1) return;
   float x[E];
   float M, L;
@@ -779,20 +786,20 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = L;
   } else {
-    const size_t p0 = (size_t)row * a.n_splits;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
+    const size_t p0 = (size_t)parts.y * heads + h % G % per_group;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;       // (the parts' are `heads` apart)
     const float* po = a.part_o + p0 * D + lane * E;
     const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
     float2 mine = make_float2(-INFINITY, 0.f);        // of split `lane` of the first 32 (of 32 at a time, below)
-    if (lane < n) mine = ml[lane];
+    if (lane < n) mine = ml[(size_t)lane * heads];
     M = mine.x;
-    for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
+    for (int s = 32 + lane; s < n; s += 32) M = fmaxf(M, ml[(size_t)s * heads].x);
     M = fmaxf(warp_max(M), sk);
     L = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = 0.f;
     for (int s0 = 0; s0 < n; s0 += 32) {
-      if (s0 > 0) mine = s0 + lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+      if (s0 > 0) mine = s0 + lane < n ? ml[(size_t)(s0 + lane) * heads] : make_float2(-INFINITY, 0.f);
       // (a maximum drops NaN, so a split that saw nothing but NaN has the factor 0 and a sum that is NaN: it has to stay)
       const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - M);
       L += mine.y * f;
@@ -802,7 +809,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4At
         float v[8][E];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const float* from = po + (size_t)(s0 + min(s + u, here - 1)) * D;
+          const float* from = po + (size_t)(s0 + min(s + u, here - 1)) * heads * D;
           if constexpr (E == 4) {
             const float4 w = *reinterpret_cast<const float4*>(from);
             v[u][0] = w.x, v[u][1] = w.y, v[u][2] = w.z, v[u][3] = w.w;
@@ -981,6 +988,7 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
   }
   __syncthreads();
   // keys beyond the caller's bound of the lengths make the row NaN (merged by the second kernel, pieces says so)
+  const int pair = row * gridDim.y + blockIdx.y;
   const bool beyond = a.shared == 2 && list.n > a.per * a.n_splits;
   for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
     const int head = i / D, d = i % D;
@@ -994,20 +1002,20 @@ __global__ void __launch_bounds__(KV4_F32_WARPS * 32) kv4_f32_kernel(const Kv4At
       L += red_ml[w][head][1] * f;
       O += red_o[w][head][d] * f;
     }
-    const size_t at = (size_t)row * a.nq + h0 + head;
     if (a.shared == 2) {
       q_s[head][d] = beyond ? __int_as_float(0x7fffffff) : O;           // (the queries are done with)
       if (d == 0) ml_s[head] = make_float2(beyond ? 0.f : M, L);
     } else if (alone) {
       finish_row<float>(a, row, live, h0 + head, d, D, M, L, O);
     } else {
-      a.part_o[(at * a.n_splits + split) * D + d] = O;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.n_splits + split) * 2) = make_float2(M, L);
+      const size_t at = ((size_t)pair * a.n_splits + split) * min(HC, G) + head;
+      a.part_o[at * D + d] = O;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
     }
   }
   if (a.shared == 2) finish_cluster<float>(a, &q_s[0][0], ml_s, row, live, h0, heads, D, split);
   else if (a.n_splits > 1 && split == 0 && threadIdx.x == 0)
-    a.pieces[(size_t)row * gridDim.y + blockIdx.y] = max(1, (list.n + a.per - 1) / a.per);
+    a.pieces[pair] = make_int2(max(1, (list.n + a.per - 1) / a.per), a.part(pair, 0));
 }
 
 // ---------------------------------------------------------------- the weights that tokens gather

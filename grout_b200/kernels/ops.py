@@ -1978,6 +1978,12 @@ def kv4_split_plan_f32(pairs: int, keys: int, sms: int) -> Tuple[int, int, int]:
     return splits, per, 2 if 1 < splits <= 8 and KV4_SHARE_OVERRIDE in (None, 2) else 0
 
 
+def kv4_parts(pairs: int, splits: int, way: int, sms: int) -> int:
+    """Parts that a call's pairs can be in: blocks that share the keys out make as many as there are blocks and pairs,
+    whatever the bound of the lengths; otherwise every pair has its splits."""
+    return KV4_PER_SM * sms + pairs if way == 1 else pairs * splits
+
+
 def _kv4_query(q, pages, block_table, step, page: int, scale, softcap, window, keep_first, chunk):
     """The checks that everything shares that takes queries over a 4-bit cache: (device, sizes, addresses, terms)."""
     dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
@@ -2060,8 +2066,8 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         ns, per, way = kv4_split_plan(n_seqs, n_seqs * groups, keys, max_pages, sms)
     po = pm = pc = 0
     if ns > 1 and way != 2:      # (memory of this call's own: two captured graphs, or two streams, share none of it)
-        n = T * nq * ns
-        part = q.new_empty(n * (D + 2) + T * groups, dtype=_F32)
+        n = kv4_parts(T * groups, ns, way, sms) * min(each, nq // nkv)
+        part = q.new_empty(n * (D + 2) + 2 * T * groups, dtype=_F32)
         po = part.data_ptr()
         pm = po + 4 * n * D
         pc = pm + 8 * n

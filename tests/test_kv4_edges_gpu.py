@@ -1,5 +1,6 @@
 """Where the operators on a 4-bit cache could go wrong: at the edges of what they are given."""
 import math
+import types
 
 import pytest
 import torch
@@ -218,3 +219,30 @@ def test_eviction_of_tokens_that_no_page_holds(place):
                 assert bool(got[j, [h, 2 + h]].isnan().all()) and w == 0.0
             else:
                 assert torch.equal(got[j, [h, 2 + h]], good[p, [h, 2 + h]])
+
+
+# ---------------------------------------------------------------- workspaces
+def peak(call):
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("n_seqs,nq,nkv,bound", [(64, 64, 8, 32768), (200, 32, 8, 8192), (256, 16, 2, 32768), (3, 12, 1, 9000)])
+def test_the_workspace_goes_by_the_parts(n_seqs, nq, nkv, bound):
+    """Blocks that share the keys out make as many parts as there are blocks and pairs, whatever the bound of the lengths."""
+    D = 64
+    pages = ops.kv4_pages(4, nkv, D, DEV)
+    table = torch.zeros((n_seqs, bound // 64 + 1), dtype=torch.int32, device=DEV)
+    lens = [1 + 37 * i % 500 for i in range(n_seqs)]
+    step = types.SimpleNamespace(slots=ints(*range(n_seqs)), kv_len=ints(*lens), cu_q=ints(*range(n_seqs + 1)), decode=True,
+                                 max_kv_len=bound, q_lens=(1,) * n_seqs)
+    q = torch.randn((n_seqs, nq, D), device=DEV).bfloat16()
+    blocks, groups = ops.KV4_PER_SM * torch.cuda.get_device_properties(0).multi_processor_count, nkv * -(-nq // nkv // 8)
+    call = lambda: ops.attention_kv4(q, pages, table, step=step, page=64, scale=0.1)
+    call()
+    most = (blocks + n_seqs * groups) * min(8, nq // nkv) * (D + 2) * 4 + q.nbytes + (1 << 20)
+    assert peak(call) <= most
