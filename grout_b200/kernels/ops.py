@@ -156,10 +156,11 @@ def _cost_attention(out, q, k_pages, *args, **kw):
     return _attention_cost(out, q, 2 * k_pages.shape[1] * q.shape[2] * k_pages.element_size(), **kw)
 
 
-def _attention_cost(out, q, token_bytes: int, **kw):
+def _attention_cost(out, q, token_bytes: int, products: int = 2, last: int = 0, **kw):
     """Keys and values of the live sequences once, q in, the result out; flops of
     the two products over the keys every query row sees (lengths are on the
-    device: they are read when the report is made)."""
+    device: they are read when the report is made).  ``products``: how many there are;
+    ``last``: only a sequence's last rows take part."""
     nq, D = q.shape[1], q.shape[2]
     kv_len, slots, cu_q, window = kw.get("kv_len"), kw.get("slots"), kw.get("cu_q"), kw.get("window")
     chunk = kw.get("chunk")
@@ -171,6 +172,8 @@ def _attention_cost(out, q, token_bytes: int, **kw):
         rows = torch.where(live, cu_q[1:] - cu_q[:-1], torch.zeros_like(kv_len)).double()
     else:
         rows = live.double()
+    if last:
+        rows = torch.clamp(rows, max=float(last))
     pairs = rows * (lens - rows) + rows * (rows + 1) / 2        # (query, visible key) pairs, causal
     if window:
         pairs = torch.minimum(pairs, rows * float(window))
@@ -182,8 +185,8 @@ def _attention_cost(out, q, token_bytes: int, **kw):
         lens = lens - torch.floor(first / chunk) * chunk
     kv_bytes = lens.sum() * token_bytes
     pair_sum = pairs.sum()
-    base = _nbytes(q, out)
-    return (lambda: base + float(kv_bytes.item())), (lambda: 4.0 * nq * D * float(pair_sum.item()))
+    base = rows.sum() * (_nbytes(q, out) / q.shape[0]) if last else _nbytes(q, out)
+    return (lambda: float(base) + float(kv_bytes.item())), (lambda: 2.0 * products * nq * D * float(pair_sum.item()))
 
 
 def _cost_qk_prepare(out, qkv, nq, nkv, D):
@@ -2109,9 +2112,9 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
     blocks = max(1, min(-(-step.max_kv_len // 128), -(-8 * sms // max(1, nkv * n_seqs))))
     args = _KV4_WEIGH.pack(qp, lp, p, w, table, sl, lens, cu, T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window,
                            keep_first, chunk, int(last), scale_log2, cap_log2, cap_inv)
-    # (the keys with their pairs, and the weights in and out)
-    cost = _PROFILE and _attention_cost(lse, q, nkv * (5 * D // 8 + 8), kv_len=step.kv_len, slots=step.slots, cu_q=step.cu_q,
-                                        window=window, chunk=chunk)
+    # (the keys' codes with their pairs, and the weights in and out)
+    cost = _PROFILE and T and _attention_cost(lse, q, nkv * (9 * D // 16 + 8), 1, int(last), kv_len=step.kv_len, slots=step.slots,
+                                              cu_q=step.cu_q, window=window, chunk=chunk)
     _launch(dev, "kv4_weigh", 1 if T else 0, cost, _fn("attn_kv4", "gb_kv4_weigh", "piip"), args, D, blocks)
 
 

@@ -148,3 +148,23 @@ def test_more_sequences_than_share_the_keys_out(least, way, monkeypatch):
     c = Cache(lens, 1, 64, BF16, seed=6)
     attend(c, [1] * 300, 2, BF16, pad=2)
     assert ops.kv4_split_plan(256, 256, 2600, 42, sms)[2] == (1 if way != 0 else 0)
+
+
+# ---------------------------------------------------------------- the profile
+def test_what_the_profile_counts_for_the_weights():
+    """Of a token and kv head the key's codes and pairs, 9 D / 16 bytes, and the weight in and out; one product."""
+    c = Cache([200, 30], 2, 64, BF16, weights=True)
+    prof = ops.OpProfile()
+    for q_lens, last in (([1, 1], 0), ([50, 20], 8)):
+        step = c.step(q_lens)
+        q = queries(sum(q_lens), 8, 64, BF16, 0).to(DEV)
+        out, lse = ops.attention_kv4(q, c.pages, c.table, step=step, page=64, scale=0.1, want_lse=True)
+        ops.set_profile(prof)
+        try:
+            ops.kv4_weigh(q, lse, c.pages, c.weights, c.table, step=step, page=64, scale=0.1, last=last)
+        finally:
+            ops.set_profile(None)
+    rows = 2 + 2 * 8
+    pairs = 230 + sum(range(193, 201)) + sum(range(23, 31))
+    calls, _ms, moved, flops = prof.totals()["kv4_weigh"]
+    assert (calls, moved, flops) == (2, 2 * 230 * 2 * (36 + 8) + rows * 8 * (128 + 4), 2.0 * 8 * 64 * pairs)
