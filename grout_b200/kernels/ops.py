@@ -1807,6 +1807,7 @@ def attention(q, k_pages, v_pages, block_table, *, step, page: int, scale: float
 _TC_ERROR_NAMES[141] = "a warp of the 4-bit decode attention waited 2 s for keys that never arrived"
 KV4_PAGE = 64              # tokens of a page
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+_I32_MOST = 0x7FFFFFFF     # (windows, chunks and bounds beyond it reach no further)
 
 
 def kv4_record(D: int) -> int:
@@ -2008,6 +2009,7 @@ def _kv4_query(q, pages, block_table, step, page: int, scale, softcap, window, k
         raise KernelError("a scale is positive; a cap, a window, a chunk and a number of kept first keys are not negative, "
                           "and chunks go without kept first keys")
     n_slots, max_pages = block_table.shape
+    window, keep_first, chunk = min(window, _I32_MOST), min(keep_first, _I32_MOST), min(chunk, _I32_MOST)
     return dev, (T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, D), (qp, p, table, sl, lens, cu), (
         window, keep_first, chunk, scale * _LOG2E, softcap * _LOG2E, scale / softcap if softcap else 0.0)
 
@@ -2062,7 +2064,7 @@ def attention_kv4(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
             raise KernelError(f"token_seq has {step.token_seq.shape[0]} entries for {T} rows")
     each = 4 if f32 else 8
     groups = nkv * ((nq // nkv + each - 1) // each)
-    keys = _keys_visited(step.max_kv_len, window, page, keep_first, chunk)
+    keys = _keys_visited(min(step.max_kv_len, max_pages * KV4_PAGE), window, page, keep_first, chunk)
     if f32:
         ns, per, way = kv4_split_plan_f32(T * groups, keys, sms)
     else:
@@ -2111,7 +2113,7 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
     sms = _SM_COUNT.get(dev) or _sm_count(q.device)
     blocks = max(1, min(-(-step.max_kv_len // 128), -(-8 * sms // max(1, nkv * n_seqs))))
     args = _KV4_WEIGH.pack(qp, lp, p, w, table, sl, lens, cu, T, n_seqs, n_slots, nq, nkv, max_pages, n_pages, window,
-                           keep_first, chunk, int(last), scale_log2, cap_log2, cap_inv)
+                           keep_first, chunk, min(int(last), _I32_MOST), scale_log2, cap_log2, cap_inv)
     # (the keys' codes with their pairs, and the weights in and out)
     cost = _PROFILE and T and _attention_cost(lse, q, nkv * (9 * D // 16 + 8), 1, int(last), kv_len=step.kv_len, slots=step.slots,
                                               cu_q=step.cu_q, window=window, chunk=chunk)

@@ -246,3 +246,28 @@ def test_the_workspace_goes_by_the_parts(n_seqs, nq, nkv, bound):
     call()
     most = (blocks + n_seqs * groups) * min(8, nq // nkv) * (D + 2) * 4 + q.nbytes + (1 << 20)
     assert peak(call) <= most
+
+
+# ---------------------------------------------------------------- numbers without a bound
+@pytest.mark.parametrize("n_rows", [1, 30])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_windows_and_bounds_beyond_32_bits(dtype, n_rows):
+    """They are windows and bounds that reach everything."""
+    c = Cache([300, 90], 2, 64, dtype, seed=7, weights=True)
+    step, q = c.step([n_rows, n_rows]), queries(2 * n_rows, 8, 64, dtype, 0).to(DEV)
+    call = lambda **seen: ops.attention_kv4(q, c.pages, c.table, step=step, page=64, scale=0.1, want_lse=True, **seen)
+    want, want_lse = call()
+    for seen in (dict(window=1 << 40), dict(window=(1 << 31) - 1), dict(window=20, keep_first=1 << 40), dict(chunk=1 << 40)):
+        out, lse = call(**seen)
+        # (another way through the kernel may add in another order: two results of which each is within half a unit)
+        assert float((out.double() - want.double()).abs().max()) <= torch.finfo(dtype).eps * 4
+        assert float((lse - want_lse).abs().max()) <= 2.0 ** -16
+    step.max_kv_len = 1 << 40
+    out, lse = call()
+    assert float((out.double() - want.double()).abs().max()) <= torch.finfo(dtype).eps * 4
+    if dtype == BF16:
+        a, b = torch.zeros_like(c.weights), torch.zeros_like(c.weights)
+        ops.kv4_weigh(q, lse, c.pages, a, c.table, step=step, page=64, scale=0.1, last=1 << 40)
+        step.max_kv_len = 300
+        ops.kv4_weigh(q, lse, c.pages, b, c.table, step=step, page=64, scale=0.1)
+        assert torch.equal(a, b)
