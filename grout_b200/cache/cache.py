@@ -96,7 +96,8 @@ class SequenceCache:
         """Cuts the sequences in ``slots`` that hold more than ``keep`` tokens to ``keep``: every kv head of every layer
         keeps their ``first`` tokens, their ``recent`` newest, and of the others those that were paid the most attention.
         The next token of such a sequence keeps its position (``dropped`` tells it from its place).  Refused, before
-        anything is changed, unless all stores of keys and values are in 4 bits, keep weights and are whole."""
+        anything is changed, unless all stores of keys and values are in 4 bits, keep weights and are whole; the memory that
+        it takes is taken before, too."""
         keep, recent, first = int(keep), int(recent), int(first)
         if keep < 1 or recent < 0 or first < 0 or first + recent > keep:
             raise ValueError(f"{first} first and {recent} recent tokens do not fit {keep} that are kept")
@@ -108,8 +109,9 @@ class SequenceCache:
         if not slots:
             return
         lengths = [self.length[s] for s in slots]
-        for st in self.stores:
-            st.evict(slots, lengths, keep, recent, first)
+        cuts = [st.prepare_evict(slots, lengths, keep, recent, first) for st in self.stores]
+        for cut in cuts:
+            cut()
         for s, n in zip(slots, lengths):
             self.length[s] = keep
             self.dropped[s] += n - keep

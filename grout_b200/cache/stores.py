@@ -178,20 +178,26 @@ class Kv4Store(KVStore):
             raise ValueError("tokens are let go of by weight from a cache that keeps weights and has neither a window "
                              f"nor chunks, not from {self.spec}")
 
-    def evict(self, slots: List[int], lengths: List[int], keep: int, recent: int, first: int) -> None:
+    def prepare_evict(self, slots: List[int], lengths: List[int], keep: int, recent: int, first: int):
         """Cuts sequences of more than ``keep`` tokens to ``keep`` in every layer (``ops.kv4_evict``) and gives the
-        pages behind them back."""
+        pages behind them back, when what is returned is called; the memory for it is taken before."""
+        memory = None
         if self.pages is not None:
             from ..kernels import ops
             self.flush()
             where, lens = (torch.tensor(x, dtype=torch.int32, device=self.device) for x in (slots, lengths))
-            for pages, weights in zip(self.pages, self.weights):
-                ops.kv4_evict(pages, weights, self.table_dev, slots=where, kv_len=lens, page=PAGE_TOKENS, keep=keep,
-                              recent=recent, first=first)
-        for slot in slots:
-            pages = self.pages_of[slot]
-            self.pool.release_many(pages[pages_for(keep):])
-            del pages[pages_for(keep):]
+            memory = ops.kv4_evict_memory(len(slots), self.spec.n_kv_heads, self.spec.head_dim, keep, self.device)
+
+        def cut() -> None:
+            if memory is not None:
+                for pages, weights in zip(self.pages, self.weights):
+                    ops.kv4_evict(pages, weights, self.table_dev, slots=where, kv_len=lens, page=PAGE_TOKENS, keep=keep,
+                                  recent=recent, first=first, memory=memory)
+            for slot in slots:
+                pages = self.pages_of[slot]
+                self.pool.release_many(pages[pages_for(keep):])
+                del pages[pages_for(keep):]
+        return cut
 
 
 class StateStore:
@@ -220,8 +226,8 @@ class StateStore:
     def check_evict(self) -> None:
         pass
 
-    def evict(self, slots, lengths, keep, recent, first) -> None:
-        pass                     # (a state has no tokens to let go of)
+    def prepare_evict(self, slots, lengths, keep, recent, first):
+        return lambda: None      # (a state has no tokens to let go of)
 
     def close(self, slot: int) -> None:
         self.open_slots.remove(slot)
@@ -262,9 +268,9 @@ class SideBySideStore:
         for st in self.stores:
             st.check_evict()
 
-    def evict(self, slots, lengths, keep, recent, first) -> None:
-        for st in self.stores:
-            st.evict(slots, lengths, keep, recent, first)
+    def prepare_evict(self, slots, lengths, keep, recent, first):
+        cuts = [st.prepare_evict(slots, lengths, keep, recent, first) for st in self.stores]
+        return lambda: [cut() for cut in cuts]
 
     def close(self, slot: int) -> None:
         for st in self.stores:

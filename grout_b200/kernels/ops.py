@@ -2123,9 +2123,19 @@ def kv4_weigh(q: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, weights: 
 _KV4_CHOOSE, _KV4_MOVE = struct.Struct("@6P8i"), struct.Struct("@8P8i")
 
 
+def kv4_evict_memory(n_seqs: int, nkv: int, D: int, keep: int, device) -> Tuple[torch.Tensor, ...]:
+    """All that ``kv4_evict`` of so many sequences in place takes from the allocator: the places kept, the new lengths,
+    records and weights on their way."""
+    records = (keep + 15) // 16
+    return (torch.empty((n_seqs, nkv, keep), dtype=_I32, device=device), torch.empty((n_seqs,), dtype=_I32, device=device),
+            torch.empty((n_seqs, nkv, records, kv4_record(D)), dtype=torch.uint8, device=device),
+            torch.empty((n_seqs, nkv, records * 16), dtype=_F32, device=device))
+
+
 def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, *, slots: torch.Tensor,
               kv_len: torch.Tensor, page: int, keep: int, recent: int, first: int = 0,
-              into: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+              into: Optional[torch.Tensor] = None,
+              memory: Optional[Tuple[torch.Tensor, ...]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Cuts sequences of more than ``keep`` tokens to ``keep``: every kv head keeps the sequence's ``first`` tokens, its
     ``recent`` newest, and of the others those with the largest ``weights`` (``kv4_weigh``; the earlier of equal ones, a
     NaN above everything).  The kept tokens move to places 0 .. keep - 1 in the order in which they stood, with their
@@ -2134,7 +2144,8 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     int32 [sequences]).  Sequences of slot -1 keep nothing, shorter ones all they have.  ``into``: a block table like
     ``block_table`` whose pages take the kept tokens (pages that no sequence of the call reads from); without it they
     stay in the sequence's first pages.  A token that no page holds is kept as NaN without a weight.  A slot must not
-    appear twice."""
+    appear twice.  ``memory``: ``kv4_evict_memory`` of these sizes, which calls in a row may share (what the one before
+    returned is then overwritten), so that a call in place allocates nothing."""
     dev, p, n_pages, nkv, D = _kv4_pages_of(pages, page)
     w = _take_weights(weights, n_pages, nkv, dev)
     table = _take(block_table, "block table", _I32, 2, dev)
@@ -2151,8 +2162,20 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
         if into.shape[0] != n_slots or to_max * KV4_PAGE < min(keep, max_pages * KV4_PAGE):
             raise KernelError(f"the block table of the kept tokens is {tuple(into.shape)} for {keep} tokens of "
                               f"{n_slots} slots")
-    kept = slots.new_empty((n_seqs, nkv, keep))
-    new = slots.new_empty((n_seqs,))
+    held = w_held = None
+    if memory is not None:
+        kept, new, held, w_held = memory
+        records = (keep + 15) // 16
+        for t, name, dtype, shape in ((kept, "places kept", _I32, (n_seqs, nkv, keep)), (new, "new lengths", _I32, (n_seqs,)),
+                                      (held, "records on their way", torch.uint8, (n_seqs, nkv, records, 18 * D)),
+                                      (w_held, "weights on their way", _F32, (n_seqs, nkv, records * 16))):
+            _take16(t, name, dtype, len(shape), dev)
+            if t.shape != shape:
+                raise KernelError(f"{name} are {tuple(t.shape)}, expected {shape}")
+    elif to_table != table:
+        kept, new = slots.new_empty((n_seqs, nkv, keep)), slots.new_empty((n_seqs,))
+    else:
+        kept, new, held, w_held = kv4_evict_memory(n_seqs, nkv, D, keep, pages.device)
     if n_seqs == 0:
         return kept, new
     choose = _KV4_CHOOSE.pack(w, table, sl, lens, kept.data_ptr(), new.data_ptr(), n_seqs, n_slots, nkv, max_pages, n_pages,
@@ -2163,10 +2186,7 @@ def kv4_evict(pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     if to_table != table:
         _launch(dev, "kv4_evict", 2, cost, evict, choose, _KV4_MOVE.pack(p, p, w, w, table, to_table, *rest, max_pages, to_max, 0),
                 None, D)
-    else:      # by way of memory of this call's own: tokens move within the pages that others are read from
-        records = (keep + 15) // 16
-        held = torch.empty((n_seqs, nkv, records, pages.shape[3]), dtype=torch.uint8, device=pages.device)
-        w_held = torch.empty((n_seqs, nkv, records * 16), dtype=_F32, device=pages.device)
+    else:      # by way of that memory: tokens move within the pages that others are read from
         h, wh = held.data_ptr(), w_held.data_ptr()
         _launch(dev, "kv4_evict", 3, cost, evict, choose, _KV4_MOVE.pack(p, h, w, wh, table, 0, *rest, max_pages, 0, 0),
                 _KV4_MOVE.pack(h, p, wh, w, 0, table, *rest, 0, max_pages, 1), D)
