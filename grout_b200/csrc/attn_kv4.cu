@@ -161,9 +161,9 @@ __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast
 // The eight codes of a word less 8, as four registers of two half-precision numbers (elements 2 i and 2 i + 1; exact).
 // A nibble in the low bits of 1024's mantissa is 1024 + c, in the next four 1024 + 16 c, so that a word takes one shift
 // and four logical operations, and the multiply-adds that take the rest off run beside them in the other pipe.  (The
-// logical pipe has half the rate and bounds these kernels: as bfloat16 numbers, 1 + c / 16, a word takes eight of it.)
+// logical pipe has half the rate and is the busiest of these kernels: as bfloat16 numbers, 1 + c / 16, a word takes eight of it.)
 // `magic` is 1024 in both halves, from kv4_magic(): an instruction takes one constant, and with two of them the compiler
-// makes two instructions of every one of these (144 of them a record instead of 72).
+// makes two instructions of every one of these (144 logical operations a record were counted, then 84; 64 are these masks).
 #define KV4_1024 0x64006400u
 __device__ __forceinline__ uint32_t kv4_magic(int not_negative) { return KV4_1024 ^ (uint32_t)(not_negative >> 31); }
 template <uint32_t MASK>
@@ -313,11 +313,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // 1 us faster on the case below, 4 % with many short sequences, and lost all of the others' values beside one 10^9 times as
 // large.)  Values are their codes less 8, so the rounding of P (2^-11) meets elements around the middle of their range;
 // m + 8 s times P is summed in 32 bits.
-// What bounds it: instructions, not memory.  A record of 16 tokens of a head takes a warp 403 of them, 288 of which are
-// its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products); four warps
-// a scheduler issue on 62 % of the cycles, the logical pipe is busy for 47 %, and the memory gives 3.2 TB/s of 6.45
-// (60 sequences of up to 4,096 keys, 32 heads of 128 on 8: 50.6 us, 26.7 at the memory's rate).  Three blocks an SM with
-// 168 registers and no spills are no faster.
+// What bounds it: nothing alone.  60 sequences of up to 4,096 keys, 32 heads of 128 on 8, take 52.2 us: 172 MB at 3.3 TB/s
+// of 6.45 (26.7 us at the memory's rate).  A record of 16 tokens of a head takes a warp 409 instructions, some 290 of which
+// are its own arithmetic (64 logical operations and 64 half-precision ones unpack 4,096 codes, 16 are products): 27 us if
+// every scheduler issued on every cycle, and four warps a scheduler issue on 61 % of them, with the logical pipe busy for
+// 46 %.  The rest is waiting inside a warp (scores, exponentials and second product of a stretch follow one another),
+// blocks that end at different times (the SMs were at work for 64 to 92 thousand cycles, 84 on average) and the merge.
+// Three blocks an SM with 168 registers and no spills are no faster.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__(Kv4Decode<D>::WARPS * 32, 4) kv4_decode_kernel
 // out[row] from the partial results of its splits, in their order; a warp a (row, head): its lanes take the splits'
 // factors first, a split a lane, and then D / 32 elements each through all splits.  Rows of one split are finished
 // already.  (With a thread for every element, which took the factors for itself, 60 sequences of up to 4,096 keys took
-// 53.6 us with their merging, now 50.9, and two of 32,768 29.9, now 27.8.)
+// 53.6 us with their merging, so 50.9, and two of 32,768 29.9 and 27.8.)
 #define MERGE_WARPS 4
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Kv4AttnArgs a, int per_group) {
