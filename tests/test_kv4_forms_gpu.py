@@ -168,3 +168,43 @@ def test_what_the_profile_counts_for_the_weights():
     pairs = 230 + sum(range(193, 201)) + sum(range(23, 31))
     calls, _ms, moved, flops = prof.totals()["kv4_weigh"]
     assert (calls, moved, flops) == (2, 2 * 230 * 2 * (36 + 8) + rows * 8 * (128 + 4), 2.0 * 8 * 64 * pairs)
+
+
+# ---------------------------------------------------------------- a large pool
+@pytest.mark.parametrize("D,nkv", [(128, 8), (64, 9)])
+def test_pages_beyond_four_gigabytes(D, nkv):
+    """Pages whose bytes lie more than 2^32 into the pool: every operator gives what it gives in a small pool, and the
+    pages at the front, where an offset of 32 bits would end, are as they were."""
+    small = Cache([300, 90, 65], nkv, D, BF16, seed=12, weights=True, spare_pages=4)
+    n, page = small.pages.shape[0], nkv * 4 * ops.kv4_record(D)
+    n_pages = (1 << 32) // page + 2 * n
+    if torch.cuda.mem_get_info()[0] < n_pages * page + (4 << 30):
+        pytest.skip("no room for the pool")
+    pages = torch.zeros((n_pages, nkv, 4, ops.kv4_record(D)), dtype=torch.uint8, device=DEV)
+    weights = torch.zeros((n_pages, nkv, 64), device=DEV)
+    weights[-n:] = small.weights
+    table = small.table + (n_pages - n)
+    assert int(table.min()) * page > 1 << 32
+    lens, nq = small.lens, 4 * nkv
+    seq = torch.repeat_interleave(torch.arange(3), torch.tensor(lens)).int().to(DEV)
+    pos = torch.cat([torch.arange(x) for x in lens]).int().to(DEV)
+    far = dict(small.at, block_table=table)
+    pages[-n:] = 0xFF                                               # (as Cache leaves what nobody has)
+    ops.kv4_write(small.kv.to(DEV), nkv, D, token_seq=seq, token_pos=pos, pages=pages, **far)
+    assert torch.equal(pages[-n:], small.pages)
+    for dtype in (BF16, F32):
+        a = ops.kv4_read(pages, token_seq=seq, token_pos=pos, dtype=dtype, **far)
+        assert torch.equal(a, ops.kv4_read(small.pages, token_seq=seq, token_pos=pos, dtype=dtype, **small.at))
+        for q_lens in ([1, 1, 1], [70, 3, 65]):
+            step, q = small.step(q_lens), queries(sum(q_lens), nq, D, dtype, 1).to(DEV)
+            got = ops.attention_kv4(q, pages, table, step=step, page=64, scale=0.1, want_lse=True)
+            want = ops.attention_kv4(q, small.pages, small.table, step=step, page=64, scale=0.1, want_lse=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            if dtype == BF16:
+                ops.kv4_weigh(q, got[1], pages, weights, table, step=step, page=64, scale=0.1)
+                ops.kv4_weigh(q, got[1], small.pages, small.weights, small.table, step=step, page=64, scale=0.1)
+                assert torch.equal(weights[-n:], small.weights)
+    cut = dict(slots=ints(*small.slots), kv_len=ints(*lens), page=64, keep=80, recent=10)
+    got, want = ops.kv4_evict(pages, weights, table, **cut), ops.kv4_evict(small.pages, small.weights, small.table, **cut)
+    assert torch.equal(got[0], want[0]) and torch.equal(pages[-n:], small.pages) and torch.equal(weights[-n:], small.weights)
+    assert not bool(pages[:-n].view(-1, 1152).any()) and not bool(weights[:-n].any())
